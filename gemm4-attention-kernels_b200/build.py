@@ -19,7 +19,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(CSRC, "libsplitd_attn.so")
 SOURCES = ["capi.cu", "fwd_kernel.cu", "bwd_preprocess.cu", "bwd_pds2_kernel.cu", "bwd_grad_kernel.cu",
-           "no_alloc.cu", "wait_probe.cu"]
+           "no_alloc.cu", "wait_probe.cu", "paged_capi.cu", "paged_attn_kernel.cu", "rotary_kernel.cu", "evict_kernel.cu"]
 
 
 def _nvcc() -> str:

@@ -61,6 +61,12 @@ size_t bwd_workspace_bytes_for(const splitd_params* p, size_t plane_limit);
 int plan_bwd(const splitd_params* p, BwdPlan& pl);
 void plan_chunk(const BwdPlan& pl, int i, const splitd_params* p, BwdParams& bp);
 int fill_bwd_params(const splitd_params* p, BwdParams& bp, const BwdPlan* pl);
+// operators on a paged cache, and rotary positions
+int launch_paged_attn(const splitd_paged_params* p, cudaStream_t stream);
+size_t paged_workspace_bytes(const splitd_paged_params* p);
+int launch_rotary(const splitd_rotary_params* p, cudaStream_t stream);
+int launch_paged_append(const splitd_append_params* p, cudaStream_t stream);
+int launch_evict(const splitd_evict_params* p, cudaStream_t stream);
 int check_common(const splitd_params* p, bool backward);
 int check_device();
 void clear_error();

@@ -1,0 +1,796 @@
+// Attention of a few query tokens per sequence over a paged cache (head_dim 512): o = softmax(q K^T scale) V, lse, and
+// optionally the attention weight that every cached key received.
+//
+// Mathematics. For one KV head, R = seqlen_q * (heads_q / heads_kv) query rows share its keys. With x = q.k scale
+// log2(e) (after the soft cap and the mask) a row keeps m = max x, l = sum 2^(x - m), O = sum 2^(x - m) v over the keys
+// seen so far; two such triples of disjoint key sets join to one by scaling both to the larger m. o = O / l and
+// lse = (m + log2 l) ln 2; a row that sees no key has l = 0: o = 0, lse = -inf.
+//
+// What bounds it. Every visible key costs 2 KB of cache and 4 * 512 * R flops: at R = 8, 8 flops a byte, far left of
+// the ridge. So the kernel is built around the stream of cache rows: one CTA per SM, a producer warp that keeps a ring
+// of six 32-row stages (200 KB) full with one 1 KB bulk copy per row (a page of any size and a row of any page is
+// then the same thing: no tile has to match a page), and eight warps that have about four times the time they need.
+//
+// Split. The (sequence, KV head, row block) units are laid end to end, in tiles of 32 keys, and every CTA takes an
+// equal share of the whole line, whatever the lengths are; the lengths never leave the device. A unit that lies inside
+// one CTA is finished there. Each CTA has at most two unfinished ones (its first and its last), whose (m, l, O) go to
+// the workspace in fp32, and the join kernel adds them up in CTA order: no atomics, the same bits every time.
+//
+// Products. keys x rows on the warp matrix instruction (16 keys x 8 rows x 16): the cache row is the A operand, so a
+// group of 8 query heads fills the 8 columns exactly. S^T = K Q^T is split over two key halves and four quarters of
+// the head dimension; the four partial sums meet in shared memory, where warp w then owns the softmax of rows w,
+// w + 8, ... with one key per lane. O^T = V^T P^T is split over the head dimension, 64 columns per warp, accumulators
+// in registers. P is kept as the sum of TWO 16-bit numbers (two products): a single one would put an error of the size
+// of the output's own rounding on top of it.
+#include <cstring>
+
+#include "launch.cuh"
+#include "paged.cuh"
+#include "warp_mma.cuh"
+
+namespace sd {
+
+namespace pa {
+constexpr int kTile = 32;                      // keys per tile = rows per ring stage
+constexpr int kStages = 6;
+constexpr int kPitch = kRowBytes + 16;         // ldmatrix reads 8 rows at once: 16 bytes of padding spread them over the banks
+constexpr int kStageBytes = kTile * kPitch;
+constexpr int kConsumers = 256;                // threads of the eight warps that compute
+constexpr int kThreads = kConsumers + 32;
+constexpr int kPartPitch = 36;                 // floats per row of the partial scores (32 keys + padding)
+constexpr int kPPitch = 20;                    // 32-bit words per row of P (32 keys x 2 bytes + padding)
+constexpr int kMaxRows = 32;                   // rows of a row block
+
+struct Desc {  // what the producer tells the others about a stretch of tiles
+  int b, head, row0, n_tiles;  // n_tiles == 0: no more work
+  int len, first_key;          // keys [first_key, len), tile by tile
+  int slot;                    // -1: the whole unit is here; 0 / 1: partial result of this CTA to keep
+  int pad;
+};
+
+template <int kNB>
+struct Layout {
+  static constexpr int kRows = 8 * kNB;
+  static constexpr int kOffPart = kStages * kStageBytes;
+  static constexpr int kOffP = kOffPart + 4 * kRows * kPartPitch * 4;
+  static constexpr int kOffCorr = kOffP + 2 * kRows * kPPitch * 4;
+  static constexpr int kOffStat = kOffCorr + kRows * 4;
+  static constexpr int kOffDesc = kOffStat + kRows * 8;
+  static constexpr int kOffBar = kOffDesc + kStages * static_cast<int>(sizeof(Desc));
+  static constexpr int kOffAbort = kOffBar + 2 * kStages * 8;
+  static constexpr int kBytes = kOffAbort + 16;
+  static_assert(kOffDesc % 16 == 0 && kOffBar % 8 == 0 && kOffPart % 16 == 0, "alignment");
+  static_assert(kBytes <= 232448, "shared memory of an SM");
+};
+}  // namespace pa
+
+struct PagedAttnParams {
+  const uint16_t *q, *k, *v;
+  uint16_t* o;
+  float* lse;
+  PageMap map;
+  const int* seqlens;
+  int64_t q_sb, q_ss, q_sh, o_sb, o_ss, o_sh;  // elements
+  int64_t k_sp, k_ss, k_sh, v_sp, v_ss, v_sh;  // page, row of the page, head
+  int batch, sq, heads_q, heads_kv, group;
+  int rows;        // sq * group: query rows of a KV head
+  int row_blocks, rows_per_block;
+  int win_left, win_right;  // -1: unbounded
+  float scale, softcap;
+  int min_tiles;   // a CTA takes at least this many tiles
+  int max_ctas;
+  // workspace
+  float* part_o;   // [CTA][2][rows_per_block][512]
+  float2* part_ml; // [CTA][2][rows_per_block]
+  float* lse2;     // [batch][heads_kv * rows] in log2 units, only with key_weights
+  float* scores;   // [batch][heads_kv * rows][weights_len], only with key_weights
+  float* weights;
+  int64_t weights_stride;
+  int weights_len;
+  int* status;
+};
+
+// First visible key of a sequence (over all its rows) and its length; tiles start at the first visible key.
+__device__ __forceinline__ int seq_len(const PagedAttnParams& p, int b) {
+  return min(max(__ldg(p.seqlens + b), 0), page_capacity(p.map));
+}
+__device__ __forceinline__ int first_key(const PagedAttnParams& p, int len) {
+  if (p.win_left < 0) return 0;
+  const long long lo = static_cast<long long>(len) - p.sq - p.win_left;
+  return lo > 0 ? static_cast<int>(lo) : 0;
+}
+__device__ __forceinline__ int seq_tiles(const PagedAttnParams& p, int len) {
+  return (len - first_key(p, len) + pa::kTile - 1) / pa::kTile;
+}
+
+// The line of tiles: `total` over all sequences, cut into `ctas` shares; share c is [c total / ctas, (c+1) total / ctas).
+struct Line {
+  long long total;
+  int ctas;
+  __device__ __forceinline__ long long begin(int c) const { return total * c / ctas; }
+  __device__ __forceinline__ int owner(long long t) const {  // largest c with begin(c) <= t
+    return static_cast<int>(((t + 1) * ctas - 1) / total);
+  }
+};
+__device__ __forceinline__ long long warp_sum(long long v) {
+#pragma unroll
+  for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  return v;
+}
+// One warp: tiles of the sequences below `end` (all of a sequence's units).
+__device__ __forceinline__ long long tiles_before(const PagedAttnParams& p, int end, int lane) {
+  long long s = 0;
+  for (int b = lane; b < end; b += 32) s += seq_tiles(p, seq_len(p, b));
+  return warp_sum(s) * (p.heads_kv * p.row_blocks);
+}
+__device__ __forceinline__ Line make_line(const PagedAttnParams& p, long long total) {
+  Line ln;
+  ln.total = total;
+  const long long want = (total + p.min_tiles - 1) / p.min_tiles;
+  ln.ctas = want < p.max_ctas ? static_cast<int>(want) : p.max_ctas;
+  return ln;
+}
+
+namespace pa {
+
+// p >= 0 as a sum of two 16-bit numbers. The upper one is the largest that is LESS than p, so that both are positive
+// where p is: a visible infinity of V times p stays an infinity (inf * 0 and inf - inf would be NaN).
+template <bool kFp16>
+__device__ __forceinline__ void split16(float p, uint16_t& hi, uint16_t& lo) {
+  const float below = p > 0.f ? __uint_as_float(__float_as_uint(p) - 1) : p;
+  if constexpr (kFp16) {
+    const __half h = __float2half_rz(below);
+    hi = __half_as_ushort(h), lo = __half_as_ushort(__float2half_rn(p - __half2float(h)));
+  } else {
+    const __nv_bfloat16 h = __float2bfloat16_rz(below);
+    hi = __bfloat16_as_ushort(h), lo = __bfloat16_as_ushort(__float2bfloat16_rn(p - __bfloat162float(h)));
+  }
+}
+
+struct Ring {
+  uint32_t full, empty;  // barrier arrays
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == kStages) stage = 0, phase ^= 1;
+  }
+};
+
+template <int kNB>
+__device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem, Ring r, volatile int* abort_flag, int lane) {
+  using L = Layout<kNB>;
+  Desc* descs = reinterpret_cast<Desc*>(smem + L::kOffDesc);
+  const uint32_t ring0 = smem_u32(smem);
+  int used = 0;  // stages handed out
+  bool ok = true;
+  auto acquire = [&]() {
+    if (ok) ok = mbar_wait(r.empty + 8 * r.stage, r.phase ^ 1, abort_flag, p.status, ST_TIMEOUT_LOAD);
+    ok = __all_sync(0xffffffffu, ok);
+    return ok;
+  };
+  const Line line = make_line(p, tiles_before(p, p.batch, lane));
+  const int cta = blockIdx.x;
+  if (cta < line.ctas) {
+    long long t = line.begin(cta);
+    const long long t_end = line.begin(cta + 1);
+    const int units = p.heads_kv * p.row_blocks;
+    // the sequence that holds tile t: whole warps of sequences at a time, then inside one
+    long long base = 0;
+    int b = 0, len = 0, n_tiles = 0;
+    for (int b0 = 0;; b0 += 32) {
+      const int my_len = b0 + lane < p.batch ? seq_len(p, b0 + lane) : 0;
+      const int mine = seq_tiles(p, my_len);
+      long long incl = static_cast<long long>(mine) * units;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const long long o = __shfl_up_sync(0xffffffffu, incl, m);
+        if (lane >= m) incl += o;
+      }
+      const unsigned past = __ballot_sync(0xffffffffu, base + incl > t);
+      if (past) {
+        const int w = __ffs(past) - 1;
+        b = b0 + w;
+        len = __shfl_sync(0xffffffffu, my_len, w);
+        n_tiles = __shfl_sync(0xffffffffu, mine, w);
+        const long long before = __shfl_sync(0xffffffffu, incl, w) - static_cast<long long>(n_tiles) * units;
+        base += before;
+        break;
+      }
+      base += __shfl_sync(0xffffffffu, incl, 31);
+      if (b0 + 32 >= p.batch) {  // the lengths changed under the kernel: nothing to do
+        t = t_end;
+        break;
+      }
+    }
+    while (t < t_end && ok) {
+      const long long off = t - base;
+      const int unit = static_cast<int>(off / n_tiles);
+      const int tile0 = static_cast<int>(off - static_cast<long long>(unit) * n_tiles);
+      const int n = static_cast<int>(min(static_cast<long long>(n_tiles - tile0), t_end - t));
+      const int head = unit / p.row_blocks;
+      const int row0 = (unit - head * p.row_blocks) * p.rows_per_block;
+      const int n_rows = min(p.rows_per_block, p.rows - row0);
+      const int lo = first_key(p, len);
+      // query rows: one ring stage, with the description of the work in front of it
+      if (!acquire()) break;
+      {
+        const uint32_t bar = r.full + 8 * r.stage;
+        if (lane == 0) {
+          Desc d;
+          d.b = b, d.head = head, d.row0 = row0, d.n_tiles = n;
+          d.len = len, d.first_key = lo + tile0 * kTile;
+          d.slot = n == n_tiles ? -1 : (tile0 > 0 ? 0 : 1);
+          d.pad = 0;
+          descs[r.stage] = d;
+          mbar_arrive_expect_tx(bar, n_rows * kRowBytes);
+        }
+        __syncwarp();
+        if (lane < n_rows) {
+          const int i = (row0 + lane) / p.group, g = (row0 + lane) - i * p.group;
+          bulk_load(ring0 + r.stage * kStageBytes + lane * kPitch, p.q + b * p.q_sb + i * p.q_ss + (head * p.group + g) * p.q_sh,
+                    kRowBytes, bar);
+        }
+        r.next(), ++used;
+      }
+      // keys and values: lane = row of the tile; the page of the next tile is looked up one tile ahead
+      auto lookup = [&](int slot, int& page, int& row) {
+        page = -1, row = 0;
+        if (slot < len) {
+          int entry;
+          split_slot(p.map, slot, entry, row);
+          page = page_of(p.map, b, entry);
+        }
+      };
+      int slot = lo + tile0 * kTile + lane, page, row;
+      lookup(slot, page, row);
+      for (int i = 0; i < n && ok; ++i) {
+        int next_page = -1, next_row = 0;
+        if (i + 1 < n) lookup(slot + kTile, next_page, next_row);
+        const bool inside = slot < len;
+        const bool have = inside && page_ok(p.map, page);
+        if (inside && !have && p.status) atomicCAS(p.status, 0, ST_BAD_PAGE);
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, have)) * kRowBytes;
+        const uint16_t* src[2] = {p.k + page * p.k_sp + row * p.k_ss + head * p.k_sh,
+                                  p.v + page * p.v_sp + row * p.v_ss + head * p.v_sh};
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!acquire()) break;
+          const uint32_t bar = r.full + 8 * r.stage;
+          const uint32_t dst = ring0 + r.stage * kStageBytes + lane * kPitch;
+          if (!have) {  // a row that is not there counts as zeros: 0 * (what lay there) could be NaN
+            for (int c = 0; c < kRowBytes; c += 16) st_shared_v4(dst + c, 0, 0, 0, 0);
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+          __syncwarp();
+          if (have) bulk_load(dst, src[kv], kRowBytes, bar);
+          r.next(), ++used;
+        }
+        slot += kTile, page = next_page, row = next_row;
+      }
+      t += n;
+      if (t < t_end && t == base + static_cast<long long>(n_tiles) * units) {  // on to the next sequence that has keys
+        base = t;
+        do {
+          ++b;
+          len = b < p.batch ? seq_len(p, b) : 0;
+          n_tiles = seq_tiles(p, len);
+        } while (b < p.batch && n_tiles == 0);
+        if (b >= p.batch) break;
+      }
+    }
+  }
+  if (acquire()) {
+    if (lane == 0) {
+      descs[r.stage].n_tiles = 0;
+      mbar_arrive(r.full + 8 * r.stage);
+    }
+  } else {
+    // a wait was given up: let the copies in flight land before the block ends
+    for (int i = 0; i < kStages && i < used; ++i) {
+      r.phase ^= r.stage == 0;
+      r.stage = r.stage == 0 ? kStages - 1 : r.stage - 1;
+      volatile int never = 0;
+      mbar_wait_limit(r.full + 8 * r.stage, r.phase, &never, nullptr, 0, 1000ull * 1000ull * 1000ull);
+    }
+  }
+}
+
+template <bool kFp16, int kNB>
+__device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem, Ring r, volatile int* abort_flag, int warp,
+                                         int lane) {
+  using L = Layout<kNB>;
+  constexpr int kRows = L::kRows;
+  const Desc* descs = reinterpret_cast<const Desc*>(smem + L::kOffDesc);
+  float* part = reinterpret_cast<float*>(smem + L::kOffPart);
+  uint16_t* p_hi = reinterpret_cast<uint16_t*>(smem + L::kOffP);
+  uint16_t* p_lo = p_hi + kRows * kPPitch * 2;
+  const uint32_t* pw_hi = reinterpret_cast<const uint32_t*>(p_hi);
+  const uint32_t* pw_lo = reinterpret_cast<const uint32_t*>(p_lo);
+  float* corr = reinterpret_cast<float*>(smem + L::kOffCorr);
+  float2* stat = reinterpret_cast<float2*>(smem + L::kOffStat);
+  const uint32_t ring0 = smem_u32(smem);
+  const int key_half = warp & 1, d_quarter = warp >> 1;
+  const int frag_row = lane >> 2, frag_col = (lane & 3) * 2;
+  const float scale_log2 = p.scale * kLog2e;
+  const float cap_in = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
+  const float cap_out = p.softcap * kLog2e;
+
+  auto wait_full = [&]() { return mbar_wait(r.full + 8 * r.stage, r.phase, abort_flag, p.status, ST_TIMEOUT_SOFTMAX); };
+  auto release = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(r.empty + 8 * r.stage);
+    r.next();
+  };
+  auto sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+
+  while (true) {
+    bool ok = wait_full();
+    // All eight warps have to agree on whether to go on, or the ones that do would wait for the others for good.
+    int go;
+    {
+      const int mine = ok && !*abort_flag;
+      asm volatile(
+          "{\n\t.reg .pred P, Q;\n\tsetp.ne.s32 P, %1, 0;\n\tbarrier.cta.red.and.pred Q, 1, 256, P;\n\tselp.s32 %0, 1, 0, Q;\n\t}"
+          : "=r"(go)
+          : "r"(mine)
+          : "memory");
+    }
+    if (!go) return;
+    const Desc d = descs[r.stage];
+    if (d.n_tiles == 0) return;
+    // query rows as B operand: [k step][n tile][2]
+    uint32_t qf[8][kNB][2];
+    {
+      const uint32_t base = ring0 + r.stage * kStageBytes + (lane & 7) * kPitch + d_quarter * 256 + (lane >> 3) * 16;
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int ks = 0; ks < 8; ks += 2) {
+          uint32_t x[4];
+          ldmatrix_x4(base + nb * 8 * kPitch + ks * 32, x);
+          qf[ks][nb][0] = x[0], qf[ks][nb][1] = x[1], qf[ks + 1][nb][0] = x[2], qf[ks + 1][nb][1] = x[3];
+        }
+    }
+    release();
+    float o[4][kNB][4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][nb][e] = 0.f;
+    float m_row[kNB], l_row[kNB];
+    int key_lo[kNB], key_hi[kNB];  // keys [key_lo, key_hi) are visible to the rows whose softmax this warp does
+#pragma unroll
+    for (int k = 0; k < kNB; ++k) {
+      m_row[k] = -INFINITY, l_row[k] = 0.f;
+      const int row = d.row0 + warp + 8 * k;
+      if (warp + 8 * k >= p.rows_per_block || row >= p.rows) {
+        key_lo[k] = 0, key_hi[k] = 0;
+      } else {
+        const long long diag = static_cast<long long>(row / p.group) + d.len - p.sq;
+        key_lo[k] = p.win_left < 0 ? 0 : static_cast<int>(max(0ll, diag - p.win_left));
+        key_hi[k] = p.win_right < 0 ? d.len : static_cast<int>(max(0ll, min(static_cast<long long>(d.len), diag + p.win_right + 1)));
+      }
+    }
+    for (int tile = 0; tile < d.n_tiles; ++tile) {
+      // ---- partial scores: 16 keys x rows over a quarter of the head dimension
+      wait_full();
+      float s[kNB][4];
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
+      {
+        const uint32_t base =
+            ring0 + r.stage * kStageBytes + (key_half * 16 + (lane & 15)) * kPitch + d_quarter * 256 + (lane >> 4) * 16;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          uint32_t a[4];
+          ldmatrix_x4(base + ks * 32, a);
+#pragma unroll
+          for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(s[nb], a, qf[ks][nb][0], qf[ks][nb][1]);
+        }
+      }
+      release();
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb) {
+        float* dst = part + (d_quarter * kRows + nb * 8 + frag_col) * kPartPitch + key_half * 16 + frag_row;
+        dst[0] = s[nb][0], dst[kPartPitch] = s[nb][1], dst[8] = s[nb][2], dst[kPartPitch + 8] = s[nb][3];
+      }
+      sync();
+      // ---- softmax: one row per warp (and n tile), one key per lane
+      const int key = d.first_key + tile * kTile + lane;
+#pragma unroll
+      for (int k = 0; k < kNB; ++k) {
+        const int row = warp + 8 * k;
+        const float* src = part + row * kPartPitch + lane;
+        float x = (src[0] + src[kRows * kPartPitch]) + (src[2 * kRows * kPartPitch] + src[3 * kRows * kPartPitch]);
+        x = p.softcap > 0.f ? cap_out * tanhf(x * cap_in) : x * scale_log2;
+        if (key < key_lo[k] || key >= key_hi[k]) x = -INFINITY;
+        if (p.scores && key < d.len && key < p.weights_len && key_hi[k] > 0)
+          p.scores[(static_cast<int64_t>(d.b) * p.heads_kv * p.rows + d.head * p.rows + d.row0 + row) * p.weights_len + key] = x;
+        float top = x;
+#pragma unroll
+        for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+        const float m_new = fmaxf(m_row[k], top);
+        float c = 1.f, e = 0.f;
+        if (m_new != -INFINITY) {
+          c = ex2(m_row[k] - m_new);
+          e = ex2(x - m_new);
+        } else if (x != x) {
+          e = x;  // every visible score is NaN: the row has to become NaN too
+        }
+        m_row[k] = m_new;
+        l_row[k] = l_row[k] * c + e;
+        uint16_t hi, lo;
+        split16<kFp16>(e, hi, lo);
+        p_hi[row * kPPitch * 2 + lane] = hi, p_lo[row * kPPitch * 2 + lane] = lo;
+        if (lane == 0) corr[row] = c;
+      }
+      sync();
+      // ---- O^T += V^T P^T, 64 columns of the head dimension
+      wait_full();
+      {
+        float cf[kNB][2];
+        bool any = false;
+#pragma unroll
+        for (int nb = 0; nb < kNB; ++nb) {
+          cf[nb][0] = corr[nb * 8 + frag_col], cf[nb][1] = corr[nb * 8 + frag_col + 1];
+          any |= cf[nb][0] != 1.f || cf[nb][1] != 1.f;
+        }
+        if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+            for (int nb = 0; nb < kNB; ++nb) {
+              o[mt][nb][0] *= cf[nb][0], o[mt][nb][1] *= cf[nb][1];
+              o[mt][nb][2] *= cf[nb][0], o[mt][nb][3] *= cf[nb][1];
+            }
+        }
+        const uint32_t base = ring0 + r.stage * kStageBytes + ((lane & 7) + (lane >> 4) * 8) * kPitch + warp * 128 + ((lane >> 3) & 1) * 16;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          uint32_t bh[kNB][2], bl[kNB][2];
+#pragma unroll
+          for (int nb = 0; nb < kNB; ++nb) {
+            const int at = (nb * 8 + frag_row) * kPPitch + ks * 8 + (lane & 3);
+            bh[nb][0] = pw_hi[at], bh[nb][1] = pw_hi[at + 4];
+            bl[nb][0] = pw_lo[at], bl[nb][1] = pw_lo[at + 4];
+          }
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            uint32_t a[4];
+            ldmatrix_x4_trans(base + ks * 16 * kPitch + mt * 32, a);
+#pragma unroll
+            for (int nb = 0; nb < kNB; ++nb) {
+              mma_16816<kFp16>(o[mt][nb], a, bh[nb][0], bh[nb][1]);
+              mma_16816<kFp16>(o[mt][nb], a, bl[nb][0], bl[nb][1]);
+            }
+          }
+        }
+      }
+      release();
+    }
+    // ---- the stretch is done
+#pragma unroll
+    for (int k = 0; k < kNB; ++k) {
+      float l = l_row[k];
+#pragma unroll
+      for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+      const int row = warp + 8 * k;
+      if (lane == 0) {
+        stat[row] = make_float2(m_row[k], l);
+        const int unit_row = d.row0 + row;
+        if (row < p.rows_per_block && unit_row < p.rows) {
+          if (d.slot < 0) {
+            const int i = unit_row / p.group, g = unit_row - i * p.group;
+            const float l2 = l == 0.f ? -INFINITY : m_row[k] + log2f(l);
+            if (p.lse) p.lse[(static_cast<int64_t>(d.b) * p.heads_q + d.head * p.group + g) * p.sq + i] = l2 * kLn2;
+            if (p.lse2) p.lse2[(static_cast<int64_t>(d.b) * p.heads_kv + d.head) * p.rows + unit_row] = l2;
+          } else {
+            p.part_ml[(blockIdx.x * 2 + d.slot) * p.rows_per_block + row] = make_float2(m_row[k], l);
+          }
+        }
+      }
+    }
+    sync();
+#pragma unroll
+    for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = nb * 8 + frag_col + e;
+        const int unit_row = d.row0 + row;
+        if (row >= p.rows_per_block || unit_row >= p.rows) continue;
+        const int col = warp * 64 + frag_row;
+        if (d.slot < 0) {
+          const int i = unit_row / p.group, g = unit_row - i * p.group;
+          const float l = stat[row].y;
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          uint16_t* dst = p.o + d.b * p.o_sb + i * p.o_ss + (d.head * p.group + g) * p.o_sh + col;
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            dst[mt * 16] = static_cast<uint16_t>(pack2<kFp16>(o[mt][nb][e] * inv, 0.f) & 0xffffu);
+            dst[mt * 16 + 8] = static_cast<uint16_t>(pack2<kFp16>(o[mt][nb][e + 2] * inv, 0.f) & 0xffffu);
+          }
+        } else {
+          float* dst = p.part_o + (static_cast<int64_t>(blockIdx.x * 2 + d.slot) * p.rows_per_block + row) * kHeadDim + col;
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) dst[mt * 16] = o[mt][nb][e], dst[mt * 16 + 8] = o[mt][nb][e + 2];
+        }
+      }
+  }
+}
+
+template <bool kFp16, int kNB>
+__global__ void __launch_bounds__(kThreads, 1) splitd_paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  using L = Layout<kNB>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffAbort);
+  Ring r;
+  r.full = smem_u32(smem + L::kOffBar);
+  r.empty = r.full + 8 * kStages;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(r.full + 8 * i, 1);
+      mbar_init(r.empty + 8 * i, kConsumers / 32);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (warp == kConsumers / 32)
+    producer<kNB>(p, smem, r, abort_flag, lane);
+  else
+    consumer<kFp16, kNB>(p, smem, r, abort_flag, warp, lane);
+}
+
+constexpr int kJoinThreads = 512;
+constexpr int kJoinGroups = kJoinThreads / 128;
+
+// One block per output row: adds up the partial results of the CTAs that share the row's unit, or writes the row of a
+// sequence without keys. Rows whose unit lay inside one CTA are finished already.
+template <bool kFp16>
+__global__ void __launch_bounds__(kJoinThreads) splitd_paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
+  __shared__ float acc[kJoinGroups][kHeadDim];
+  __shared__ long long span[3];  // line total, first tile of this sequence, tiles of a unit of it
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hr = blockIdx.x, b = blockIdx.y;  // hr = head * rows + row of the unit's KV head
+  const int head = hr / p.rows, unit_row = hr - head * p.rows;
+  const int rb = unit_row / p.rows_per_block, row = unit_row - rb * p.rows_per_block;
+  const int units = p.heads_kv * p.row_blocks;
+  if (hr == 0 && tid == 0 && __ldg(p.seqlens + b) > page_capacity(p.map) && p.status) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
+  if (warp == 0) {
+    const long long before = tiles_before(p, b, lane);
+    long long after = 0;
+    for (int i = b + lane; i < p.batch; i += 32) after += seq_tiles(p, seq_len(p, i));
+    after = warp_sum(after) * units;
+    if (lane == 0) {
+      span[0] = before + after;
+      span[1] = before;
+      span[2] = seq_tiles(p, seq_len(p, b));
+    }
+  }
+  __syncthreads();
+  pdl_wait();
+  const int n_tiles = static_cast<int>(span[2]);
+  const int i = unit_row / p.group, g = unit_row - i * p.group;
+  const int hq = head * p.group + g;
+  uint16_t* out = p.o + b * p.o_sb + i * p.o_ss + hq * p.o_sh;
+  const int64_t lse_at = (static_cast<int64_t>(b) * p.heads_q + hq) * p.sq + i;
+  const int64_t lse2_at = static_cast<int64_t>(b) * p.heads_kv * p.rows + hr;
+  if (n_tiles == 0) {
+    for (int c = tid; c < kHeadDim; c += kJoinThreads) out[c] = 0;
+    if (tid == 0) {
+      if (p.lse) p.lse[lse_at] = -INFINITY;
+      if (p.lse2) p.lse2[lse2_at] = -INFINITY;
+    }
+    return;
+  }
+  const Line line = make_line(p, span[0]);
+  const long long t0 = span[1] + static_cast<long long>(head * p.row_blocks + rb) * n_tiles;
+  const int c0 = line.owner(t0), c1 = line.owner(t0 + n_tiles - 1);
+  if (c0 == c1) return;
+  // the first CTA's share ends inside the unit (its second partial result) unless the unit starts the share; all
+  // later CTAs begin inside the unit
+  auto slot_of = [&](int c) { return c == c0 ? 2 * c + 1 : 2 * c; };
+  float m = -INFINITY;
+  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[slot_of(c) * p.rows_per_block + row].x);
+#pragma unroll
+  for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+  const float m_ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  for (int c = c0 + lane; c <= c1; c += 32) {
+    const float2 ml = p.part_ml[slot_of(c) * p.rows_per_block + row];
+    l += ml.y * ex2(ml.x - m_ref);
+  }
+#pragma unroll
+  for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+  const int grp = tid >> 7, col = (tid & 127) * 4;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int c = c0 + grp; c <= c1; c += kJoinGroups) {
+    const int64_t at = static_cast<int64_t>(slot_of(c)) * p.rows_per_block + row;
+    const float w = ex2(p.part_ml[at].x - m_ref);
+    const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * kHeadDim + col);
+    s.x += w * v.x, s.y += w * v.y, s.z += w * v.z, s.w += w * v.w;
+  }
+  *reinterpret_cast<float4*>(&acc[grp][col]) = s;
+  __syncthreads();
+  if (grp == 0) {
+#pragma unroll
+    for (int k = 1; k < kJoinGroups; ++k) {
+      const float4 v = *reinterpret_cast<const float4*>(&acc[k][col]);
+      s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint2 w;
+    w.x = pack2<kFp16>(s.x * inv, s.y * inv), w.y = pack2<kFp16>(s.z * inv, s.w * inv);
+    *reinterpret_cast<uint2*>(out + col) = w;
+    if (tid == 0) {
+      const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
+      if (p.lse) p.lse[lse_at] = l2 * kLn2;
+      if (p.lse2) p.lse2[lse2_at] = l2;
+    }
+  }
+}
+
+constexpr int kWeightThreads = 256;
+
+// key_weights[b][j] += sum over the query rows of 2^(x - lse2), in row order. One key per thread.
+__global__ void __launch_bounds__(kWeightThreads) splitd_paged_weights_kernel(const __grid_constant__ PagedAttnParams p) {
+  const int b = blockIdx.y;
+  const int len = seq_len(p, b);
+  if (blockIdx.x == 0 && threadIdx.x == 0 && len > p.weights_len && p.status) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
+  const int n = min(len, p.weights_len);
+  const int key = first_key(p, len) + blockIdx.x * kWeightThreads + threadIdx.x;
+  pdl_wait();
+  if (key >= n) return;
+  const int rows = p.heads_kv * p.rows;
+  const float* x = p.scores + static_cast<int64_t>(b) * rows * p.weights_len + key;
+  const float* l2 = p.lse2 + static_cast<int64_t>(b) * rows;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int r = 0; r < rows; ++r) {
+    const float l = __ldg(l2 + r), v = __ldcs(x + static_cast<int64_t>(r) * p.weights_len);
+    sum += l == -INFINITY ? 0.f : ex2(v - l);
+  }
+  p.weights[b * p.weights_stride + key] += sum;
+}
+
+}  // namespace pa
+
+namespace {
+
+int row_blocks_of(int rows) { return (rows + pa::kMaxRows - 1) / pa::kMaxRows; }
+int rows_per_block_of(int rows) { return (rows + row_blocks_of(rows) - 1) / row_blocks_of(rows); }
+
+int64_t max_keys(const splitd_paged_params* p) { return static_cast<int64_t>(p->max_pages) * p->page_size; }
+
+int sm_count() {
+  static std::atomic<int> cache[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64) {
+    const int c = cache[dev].load(std::memory_order_acquire);
+    if (c > 0) return c;
+  }
+  int n = 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  if (dev >= 0 && dev < 64) cache[dev].store(n, std::memory_order_release);
+  return n;
+}
+
+constexpr int kMinTiles = 1;
+constexpr int kMaxCtas = 256;  // sizes the workspace without asking a device
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+}  // namespace
+
+size_t paged_workspace_bytes(const splitd_paged_params* p) {
+  if (p->batch <= 0 || p->seqlen_q <= 0 || p->heads_q <= 0 || p->heads_kv <= 0) return 0;
+  const int64_t rows = static_cast<int64_t>(p->seqlen_q) * (p->heads_q / p->heads_kv);
+  const size_t rpb = rows < pa::kMaxRows ? rows : pa::kMaxRows;
+  size_t n = align256(static_cast<size_t>(kMaxCtas) * 2 * rpb * kHeadDim * 4) + align256(static_cast<size_t>(kMaxCtas) * 2 * rpb * 8);
+  if (p->key_weights) {
+    const size_t all = static_cast<size_t>(p->batch) * rows * p->heads_kv;
+    n += align256(all * 4) + align256(all * p->key_weights_len * 4);
+  }
+  return n;
+}
+
+namespace {
+
+template <typename Kernel>
+int raise_smem(Kernel kern, int bytes, std::atomic<int> (&done)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire)) return 0;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(SPLITD_ERR_CUDA, "paged attention: the kernel's shared memory cannot be set");
+  }
+  if (dev >= 0 && dev < 64) done[dev].store(1, std::memory_order_release);
+  return 0;
+}
+
+template <bool kFp16, int kNB>
+int launch_main(const PagedAttnParams& p, int grid, cudaStream_t stream) {
+  static std::atomic<int> done[64];
+  auto kern = pa::splitd_paged_attn_kernel<kFp16, kNB>;
+  if (int e = raise_smem(kern, pa::Layout<kNB>::kBytes, done)) return e;
+  kern<<<grid, pa::kThreads, pa::Layout<kNB>::kBytes, stream>>>(p);
+  return 0;
+}
+
+}  // namespace
+
+int launch_paged_attn(const splitd_paged_params* a, cudaStream_t stream) {
+  PagedAttnParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = static_cast<const uint16_t*>(a->q), p.k = static_cast<const uint16_t*>(a->k_pages), p.v = static_cast<const uint16_t*>(a->v_pages);
+  p.o = static_cast<uint16_t*>(a->o), p.lse = a->lse;
+  p.map = {a->page_table, a->page_table_stride, a->max_pages, a->page_size, a->num_pages, page_shift(a->page_size)};
+  p.seqlens = a->seqlens_k;
+  p.q_sb = a->q_strides[0], p.q_ss = a->q_strides[1], p.q_sh = a->q_strides[2];
+  p.o_sb = a->o_strides[0], p.o_ss = a->o_strides[1], p.o_sh = a->o_strides[2];
+  p.k_sp = a->k_strides[0], p.k_ss = a->k_strides[1], p.k_sh = a->k_strides[2];
+  p.v_sp = a->v_strides[0], p.v_ss = a->v_strides[1], p.v_sh = a->v_strides[2];
+  p.batch = a->batch, p.sq = a->seqlen_q, p.heads_q = a->heads_q, p.heads_kv = a->heads_kv;
+  p.group = a->heads_q / a->heads_kv;
+  p.rows = p.sq * p.group;
+  p.row_blocks = row_blocks_of(p.rows), p.rows_per_block = rows_per_block_of(p.rows);
+  p.win_left = a->local ? a->window_left : -1;
+  p.win_right = a->causal ? 0 : a->local ? a->window_right : -1;
+  p.scale = a->softmax_scale, p.softcap = a->softcap;
+  p.min_tiles = kMinTiles;
+  p.status = a->status_flag;
+  // no more CTAs than tiles there can be
+  const int64_t most = static_cast<int64_t>(p.batch) * p.heads_kv * p.row_blocks * ((max_keys(a) + pa::kTile - 1) / pa::kTile);
+  int grid = sm_count() < kMaxCtas ? sm_count() : kMaxCtas;
+  if (most < grid) grid = most > 0 ? static_cast<int>(most) : 1;
+  p.max_ctas = grid;
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  p.part_o = reinterpret_cast<float*>(ws);
+  ws += align256(static_cast<size_t>(kMaxCtas) * 2 * p.rows_per_block * kHeadDim * 4);
+  p.part_ml = reinterpret_cast<float2*>(ws);
+  ws += align256(static_cast<size_t>(kMaxCtas) * 2 * p.rows_per_block * 8);
+  if (a->key_weights) {
+    const size_t all = static_cast<size_t>(p.batch) * p.rows * p.heads_kv;
+    p.lse2 = reinterpret_cast<float*>(ws);
+    ws += align256(all * 4);
+    p.scores = reinterpret_cast<float*>(ws);
+    p.weights = a->key_weights, p.weights_stride = a->key_weights_stride, p.weights_len = a->key_weights_len;
+  }
+  const bool fp16 = a->dtype == SPLITD_DTYPE_FP16;
+  const int nb = (p.rows_per_block + 7) / 8;
+  int e;
+  if (nb == 1)
+    e = fp16 ? launch_main<true, 1>(p, grid, stream) : launch_main<false, 1>(p, grid, stream);
+  else if (nb == 2)
+    e = fp16 ? launch_main<true, 2>(p, grid, stream) : launch_main<false, 2>(p, grid, stream);
+  else
+    e = fp16 ? launch_main<true, 4>(p, grid, stream) : launch_main<false, 4>(p, grid, stream);
+  if (e) return e;
+  cudaError_t ce = cudaGetLastError();
+  if (ce == cudaSuccess)
+    ce = launch_dependent(fp16 ? pa::splitd_paged_join_kernel<true> : pa::splitd_paged_join_kernel<false>,
+                          dim3(p.heads_kv * p.rows, p.batch), dim3(pa::kJoinThreads), 0, stream, p);
+  if (ce == cudaSuccess && p.weights) {
+    const int64_t longest = max_keys(a) < p.weights_len ? max_keys(a) : p.weights_len;
+    ce = launch_dependent(pa::splitd_paged_weights_kernel,
+                          dim3(static_cast<unsigned>((longest + pa::kWeightThreads - 1) / pa::kWeightThreads), p.batch),
+                          dim3(pa::kWeightThreads), 0, stream, p);
+  }
+  if (ce != cudaSuccess) {
+    cudaGetLastError();
+    return fail(SPLITD_ERR_CUDA, "paged attention: launch failed: %s", cudaGetErrorString(ce));
+  }
+  return 0;
+}
+
+}  // namespace sd

@@ -21,6 +21,8 @@ enum : int {
   ST_TIMEOUT_PEER = 104,
   ST_BAD_SMEM_ALIGN = 105,   // dynamic shared memory not 1024-byte aligned
   ST_BAD_SEQLEN = 106,       // packed layout: a sequence is longer than the max_seqlen_k the workspace was sized for
+  ST_BAD_PAGE = 107,         // paged cache: a page table names a page that the cache does not have
+  ST_BAD_CACHE_LEN = 108,    // paged cache: a sequence is longer than its row of the page table (or of key_weights)
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

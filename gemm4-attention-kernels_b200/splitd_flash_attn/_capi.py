@@ -36,6 +36,11 @@ EXPORTED_SYMBOLS = (
     "splitd_bwd_static_scratch",
     "splitd_bwd_static_scratch_limit_rowstat",
     "splitd_bwd_static_scratch_limit_workspace",
+    "splitd_paged_attn",
+    "splitd_paged_attn_workspace_bytes",
+    "splitd_rotary",
+    "splitd_paged_append",
+    "splitd_paged_evict",
     "splitd_last_error",
     "splitd_version",
 )
@@ -91,6 +96,82 @@ class SplitdParams(ctypes.Structure):
         ("o_resid", ctypes.c_void_p),
         ("o_resid_all", ctypes.c_int32),
     ]
+
+
+def _fields(text):
+    """Fields of a parameter struct, one kind per line: ``kind: name name ...``; ``name*3`` is an array."""
+    kinds = {
+        "ptr": ctypes.c_void_p,
+        "size": ctypes.c_size_t,
+        "i32": ctypes.c_int32,
+        "i64": ctypes.c_int64,
+        "f32": ctypes.c_float,
+    }
+    out = []
+    for line in text.strip().splitlines():
+        kind, names = line.split(":")
+        for name in names.split():
+            name, _, n = name.partition("*")
+            t = kinds[kind.strip()]
+            out.append((name, t * int(n) if n else t))
+    return out
+
+
+class SplitdPagedParams(ctypes.Structure):
+    """Mirror of ``splitd_paged_params``."""
+
+    _fields_ = _fields(
+        """
+        ptr: q k_pages v_pages o lse key_weights page_table seqlens_k workspace
+        size: workspace_bytes
+        ptr: status_flag
+        i32: batch seqlen_q heads_q heads_kv head_dim num_pages page_size max_pages key_weights_len dtype causal
+        i32: local window_left window_right
+        f32: softmax_scale softcap
+        i64: page_table_stride key_weights_stride q_strides*3 o_strides*3 k_strides*3 v_strides*3
+        """
+    )
+
+
+class SplitdRotaryParams(ctypes.Structure):
+    """Mirror of ``splitd_rotary_params``."""
+
+    _fields_ = _fields(
+        """
+        ptr: q k q_out k_out positions inv_freq
+        i32: batch seqlen heads_q heads_kv head_dim rotary_dim interleaved backward positions_64bit dtype
+        f32: factor
+        i64: position_strides*2 q_strides*3 k_strides*3 q_out_strides*3 k_out_strides*3
+        """
+    )
+
+
+class SplitdAppendParams(ctypes.Structure):
+    """Mirror of ``splitd_append_params``."""
+
+    _fields_ = _fields(
+        """
+        ptr: q k v q_out k_pages v_pages page_table seqlens_k cu_seqlens positions inv_freq status_flag
+        i32: batch seqlen total_tokens heads_q heads_kv head_dim num_pages page_size max_pages
+        i32: rotary_dim interleaved positions_64bit dtype
+        f32: factor
+        i64: page_table_stride position_strides*2 q_strides*3 k_strides*3 v_strides*3 q_out_strides*3
+        i64: k_page_strides*3 v_page_strides*3
+        """
+    )
+
+
+class SplitdEvictParams(ctypes.Structure):
+    """Mirror of ``splitd_evict_params``."""
+
+    _fields_ = _fields(
+        """
+        ptr: k_pages v_pages page_table new_page_table seqlens_k key_weights new_seqlens kept new_weights status_flag
+        i32: batch heads_kv head_dim num_pages page_size max_pages new_max_pages
+        i32: key_weights_len keep keep_first keep_recent
+        i64: page_table_stride new_page_table_stride key_weights_stride k_strides*3 v_strides*3
+        """
+    )
 
 
 class SplitdError(RuntimeError):
@@ -150,6 +231,17 @@ def load_library() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = []
         fn.restype = ctypes.c_size_t
+    for name, params in (
+        ("splitd_paged_attn", SplitdPagedParams),
+        ("splitd_rotary", SplitdRotaryParams),
+        ("splitd_paged_append", SplitdAppendParams),
+        ("splitd_paged_evict", SplitdEvictParams),
+    ):
+        fn = getattr(lib, name)
+        fn.argtypes = [ctypes.POINTER(params), ctypes.c_void_p]
+        fn.restype = ctypes.c_int
+    lib.splitd_paged_attn_workspace_bytes.argtypes = [ctypes.POINTER(SplitdPagedParams)]
+    lib.splitd_paged_attn_workspace_bytes.restype = ctypes.c_size_t
     lib.splitd_last_error.restype = ctypes.c_char_p
     lib.splitd_version.restype = ctypes.c_char_p
     _lib = lib

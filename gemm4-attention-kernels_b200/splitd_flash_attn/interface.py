@@ -310,7 +310,8 @@ def kernel_status(device: Optional[torch.device] = None) -> int:
 
     The kernels never spin forever: a wait that exceeds 4 s is given up, the kernel ends early and stores a
     code here (101 loads, 102 tensor-core issue, 103 softmax/epilogue, 104 peer CTA, 105 shared-memory
-    alignment, 106 a packed sequence longer than max_seqlen_k). Outputs of such a call are incomplete. The calls
+    alignment, 106 a packed sequence longer than max_seqlen_k, 107 a page table that names a page its cache does not
+    have, 108 a sequence longer than its row of the page table). Outputs of such a call are incomplete. The calls
     of this module are asynchronous, so nothing can raise at the call itself: check this after a step (it costs
     one 4-byte copy), e.g. where the loss is read. The packed API looks at it whenever it validates cu_seqlens.
     ``reset_kernel_status()`` re-arms it.

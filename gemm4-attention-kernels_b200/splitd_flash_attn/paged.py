@@ -1,0 +1,534 @@
+"""Generation with head_dim 512: a cache of keys and values in pages, the attention that reads it, the append that
+fills it and the eviction that shortens it (no counterpart in the reference, which has no cache).
+
+A cache is two tensors ``k_pages`` and ``v_pages`` of shape (num_pages, page_size, heads_kv, 512), bf16 or fp16, any page
+size. ``page_table`` (B, max_pages) int32 names the pages of each sequence, ``seqlens_k`` (B,) int32 the slots in use;
+slot j of sequence b is row ``j % page_size`` of page ``page_table[b, j // page_size]``. Both stay on the device: no call
+here waits for the GPU, and all of them can be captured in a CUDA graph. The kernels check every page id and length
+before they use it; ``kernel_status()`` is 107 or 108 after a call that named a page the cache does not have or a
+sequence longer than its row of the table.
+
+One step of a decoder's layer::
+
+    q = split_paged_append_func(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq=inv_freq)
+    out = split_flash_attn_paged_func(q, k_pages, v_pages, page_table, seqlens_k, causal=True)
+
+with ``seqlens_k`` counting the new tokens already. Kernels: ``csrc/paged_attn_kernel.cu``, ``csrc/rotary_kernel.cu``,
+``csrc/evict_kernel.cu``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _capi
+from .interface import (
+    SUPPORTED_HEAD_DIM,
+    _dec,
+    _enc,
+    _resolve_causal_local_window,
+    _status_flag,
+    _validate_cu_seqlens,
+)
+from .rotary import (
+    _DTYPES,
+    _call,
+    _check_heads,
+    _check_inv_freq,
+    _check_positions,
+    _check_same,
+    _position_strides,
+    _rows,
+    _token_strides,
+    _traced,
+)
+
+__all__ = ["split_flash_attn_paged_func", "split_paged_append_func", "split_paged_evict_func"]
+
+
+# ---------------------------------------------------------------------------
+# argument checks
+# ---------------------------------------------------------------------------
+
+
+def _check_cache(k_pages, v_pages, page_table, seqlens_k, page_table_name="page_table") -> None:
+    _check_heads(k_pages, "k_pages", 4)
+    _check_heads(v_pages, "v_pages", 4)
+    if v_pages.shape != k_pages.shape:
+        raise ValueError(f"v_pages has shape {tuple(v_pages.shape)}, expected {tuple(k_pages.shape)}")
+    device = k_pages.device
+    _check_same(v_pages, "v_pages", k_pages.dtype, device)
+    if k_pages.shape[1] == 0 or k_pages.shape[2] == 0:
+        raise ValueError(f"k_pages has shape {tuple(k_pages.shape)}: page_size and heads_kv must not be 0")
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        # a cache is not copied: its rows have to be where 16-byte accesses can reach them
+        s = t.stride()
+        if s[3] != 1 or s[0] % 8 or s[1] % 8 or s[2] % 8:
+            raise ValueError(f"{name} needs an innermost stride of 1 and other strides that are multiples of 8, got {s}")
+    if seqlens_k.ndim != 1:
+        raise ValueError(f"seqlens_k must be a 1D tensor, got rank {seqlens_k.ndim}")
+    _check_same(seqlens_k, "seqlens_k", torch.int32, device)
+    _check_table(page_table, page_table_name, seqlens_k.shape[0], device)
+
+
+def _check_table(page_table, name, batch, device) -> None:
+    if page_table.ndim != 2 or page_table.shape[0] != batch:
+        raise ValueError(f"{name} has shape {tuple(page_table.shape)}, expected ({batch}, pages per sequence)")
+    _check_same(page_table, name, torch.int32, device)
+
+
+def _check_aligned(k_pages, v_pages) -> None:
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if t.data_ptr() % 16:
+            raise ValueError(f"{name} must start at a 16-byte boundary")
+
+
+def _check_weights(key_weights, batch, device) -> None:
+    if key_weights.ndim != 2 or key_weights.shape[0] != batch:
+        raise ValueError(f"key_weights has shape {tuple(key_weights.shape)}, expected ({batch}, slots)")
+    _check_same(key_weights, "key_weights", torch.float32, device)
+    if key_weights.shape[1] > 1 and key_weights.stride(1) != 1:
+        raise ValueError("key_weights must have an innermost stride of 1")
+
+
+def _unit_rows(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+# ---------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------
+
+
+def _check_paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights) -> None:
+    _check_heads(q, "q", 4)
+    _check_cache(k_pages, v_pages, page_table, seqlens_k)
+    _check_same(k_pages, "k_pages", q.dtype, q.device)
+    if q.shape[0] != seqlens_k.shape[0]:
+        raise ValueError(f"q has shape {tuple(q.shape)}, but seqlens_k names {seqlens_k.shape[0]} sequences")
+    if q.shape[2] == 0 or q.shape[2] % k_pages.shape[2]:
+        raise ValueError(f"num_head ({q.shape[2]}) must be divisible by num_head_kv ({k_pages.shape[2]})")
+    if key_weights is not None:
+        _check_weights(key_weights, q.shape[0], q.device)
+
+
+def _paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, causal, left, right, softcap, want_lse):
+    causal, local = _resolve_causal_local_window(causal, left, right)
+    _check_aligned(k_pages, v_pages)
+    device = q.device
+    batch, sq, hq, _ = q.shape
+    q = _rows(q)
+    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    lse = torch.empty((batch, hq, sq), dtype=torch.float32, device=device) if want_lse else None
+    if out.numel() == 0:
+        return out, lse
+    page_table, seqlens_k = _unit_rows(page_table), _unit_rows(seqlens_k)
+    lib = _capi.load_library()
+    counted = key_weights is not None and key_weights.shape[1] > 0
+    params = _capi.SplitdPagedParams(
+        q.data_ptr(),
+        k_pages.data_ptr() or 256,  # a cache without pages has no memory, and none of it is touched
+        v_pages.data_ptr() or 256,
+        out.data_ptr(),
+        lse.data_ptr() if want_lse else None,
+        key_weights.data_ptr() if counted else None,
+        page_table.data_ptr() or 256,
+        seqlens_k.data_ptr(),
+        None,
+        0,
+        _status_flag(device).data_ptr(),
+        batch,
+        sq,
+        hq,
+        k_pages.shape[2],
+        SUPPORTED_HEAD_DIM,
+        k_pages.shape[0],
+        k_pages.shape[1],
+        page_table.shape[1],
+        key_weights.shape[1] if counted else 0,
+        _DTYPES[q.dtype],
+        1 if causal else 0,
+        1 if local else 0,
+        -1 if left is None or left < 0 else min(left, 2**31 - 1),
+        -1 if right is None or right < 0 else min(right, 2**31 - 1),
+        softmax_scale,
+        softcap,
+        page_table.stride(0),
+        key_weights.stride(0) if counted else 0,
+        _token_strides(q),
+        _token_strides(out),
+        k_pages.stride()[:3],
+        v_pages.stride()[:3],
+    )
+    n = lib.splitd_paged_attn_workspace_bytes(ctypes.byref(params))
+    workspace = torch.empty(n, dtype=torch.uint8, device=device)
+    params.workspace, params.workspace_bytes = workspace.data_ptr(), n
+    _call(lib.splitd_paged_attn, params, device)
+    return out, lse
+
+
+@torch.library.custom_op("splitd_flash_attn::paged_attn", mutates_args=("key_weights",))
+def _paged_attn_custom(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    page_table: torch.Tensor,
+    seqlens_k: torch.Tensor,
+    key_weights: Optional[torch.Tensor],
+    softmax_scale: float,
+    causal: bool,
+    window_size_left: int,
+    window_size_right: int,
+    softcap: float,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    _check_paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights)
+    return _paged_attn(
+        q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, causal, _dec(window_size_left),
+        _dec(window_size_right), softcap, True,
+    )
+
+
+@torch.library.register_fake("splitd_flash_attn::paged_attn")
+def _paged_attn_fake(
+    q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, causal, window_size_left, window_size_right, softcap
+):
+    _check_paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights)
+    return q.new_empty(q.shape), q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
+
+
+def split_flash_attn_paged_func(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    page_table: torch.Tensor,
+    seqlens_k: torch.Tensor,
+    softmax_scale: Optional[float] = None,
+    causal: bool = False,
+    window_size: Tuple[Optional[int], Optional[int]] = (None, None),
+    softcap: float = 0.0,
+    key_weights: Optional[torch.Tensor] = None,
+    return_lse: bool = False,
+):
+    """Attention of a few query tokens per sequence (one when decoding, a few when verifying drafted tokens) over a
+    paged cache. Forward only. Returns ``out`` or ``(out, lse)``.
+
+    q (B, Sq, Hq, 512) with Hq % heads_kv == 0, in the cache's dtype. ``seqlens_k[b]`` counts the sequence's slots with
+    its Sq new tokens: query i stands at slot ``seqlens_k[b] - Sq + i``, and ``causal``, ``window_size`` and ``softcap``
+    mean what they mean in ``split_flash_attn_func`` (bottom-right alignment; causal changes nothing for Sq = 1). A row
+    that sees no slot, as in a sequence of length 0, gets out 0 and lse -inf. Slots that no row of a sequence may see
+    are not read; one that only some of its rows may see has weight 0 in the others, like any masked key of a dense
+    product (0 times an infinity is NaN there too).
+
+    ``key_weights`` (B, slots) float32, optional: every slot's softmax weight, summed over all query heads and tokens,
+    is added to it in place, in a fixed order (what ``split_paged_evict_func`` ranks by). Costs a workspace of
+    Hq * Sq * 4 bytes per slot of it.
+
+    The cache is read once for up to 32 rows (Sq * Hq / heads_kv); more rows take as many passes.
+    """
+    if not isinstance(window_size, tuple) or len(window_size) != 2:
+        raise TypeError("window_size must be a tuple of (left, right)")
+    _check_paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights)
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        raise NotImplementedError("SplitD paged attention has no backward: call it under torch.no_grad() or detach its inputs")
+    softmax_scale = 1.0 / math.sqrt(SUPPORTED_HEAD_DIM) if softmax_scale is None else float(softmax_scale)
+    left, right = window_size
+    if _traced(q, k_pages, v_pages, page_table, seqlens_k, key_weights):
+        out, lse = torch.ops.splitd_flash_attn.paged_attn(
+            q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, bool(causal), _enc(left), _enc(right),
+            float(softcap),
+        )
+    else:
+        out, lse = _paged_attn(
+            q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, bool(causal), left, right,
+            float(softcap), return_lse,
+        )
+    return (out, lse) if return_lse else out
+
+
+# ---------------------------------------------------------------------------
+# append
+# ---------------------------------------------------------------------------
+
+
+def _check_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q) -> None:
+    rank = 4 if cu_seqlens_q is None else 3
+    _check_heads(k, "k", rank)
+    _check_heads(v, "v", rank)
+    _check_cache(k_pages, v_pages, page_table, seqlens_k)
+    if v.shape != k.shape:
+        raise ValueError(f"v has shape {tuple(v.shape)}, expected {tuple(k.shape)}")
+    if k.shape[-2] != k_pages.shape[2]:
+        raise ValueError(f"k has {k.shape[-2]} heads, the cache {k_pages.shape[2]}")
+    for name, t in (("v", v), ("k_pages", k_pages)):
+        _check_same(t, name, k.dtype, k.device)
+    if q is not None:
+        _check_heads(q, "q", rank)
+        if q.shape[:-2] != k.shape[:-2]:
+            raise ValueError(f"q has shape {tuple(q.shape)}, expected the tokens of k, {tuple(k.shape)}")
+        _check_same(q, "q", k.dtype, k.device)
+        if q.shape[-2] == 0 or q.shape[-2] % k.shape[-2]:
+            raise ValueError(f"num_head ({q.shape[-2]}) must be divisible by num_head_kv ({k.shape[-2]})")
+    batch = seqlens_k.shape[0]
+    if cu_seqlens_q is None:
+        if k.shape[0] != batch:
+            raise ValueError(f"k has shape {tuple(k.shape)}, but seqlens_k names {batch} sequences")
+    elif tuple(cu_seqlens_q.shape) != (batch + 1,):
+        raise ValueError(f"cu_seqlens_q must have shape ({batch + 1},), got {tuple(cu_seqlens_q.shape)}")
+    else:
+        _check_same(cu_seqlens_q, "cu_seqlens_q", torch.int32, k.device)
+    if inv_freq is not None:
+        _check_inv_freq(inv_freq, k.device)
+    elif positions is not None:
+        raise ValueError("positions is given without inv_freq: there is nothing to rotate")
+    if positions is not None:
+        _check_positions(positions, k.shape[:-2], k.device)
+
+
+def _paged_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q, interleaved, factor):
+    _check_aligned(k_pages, v_pages)
+    packed = cu_seqlens_q is not None
+    batch = seqlens_k.shape[0]
+    if packed:
+        _validate_cu_seqlens(cu_seqlens_q, "cu_seqlens_q", batch, total_tokens=k.shape[0])
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if k.numel() == 0:
+        return q_out
+    page_table, seqlens_k = _unit_rows(page_table), _unit_rows(seqlens_k)
+    none = (0, 0, 0)
+    pairs = 0 if inv_freq is None else inv_freq.numel()
+    if pairs:
+        inv_freq = inv_freq.contiguous()
+    lib = _capi.load_library()
+    params = _capi.SplitdAppendParams(
+        q.data_ptr() if q is not None else None,
+        k.data_ptr(),
+        v.data_ptr(),
+        q_out.data_ptr() if q is not None else None,
+        k_pages.data_ptr() or 256,  # see _paged_attn
+        v_pages.data_ptr() or 256,
+        page_table.data_ptr() or 256,
+        seqlens_k.data_ptr() or 256,
+        cu_seqlens_q.data_ptr() if packed else None,
+        positions.data_ptr() if positions is not None else None,
+        inv_freq.data_ptr() if pairs else None,
+        _status_flag(k.device).data_ptr(),
+        batch,
+        0 if packed else k.shape[1],
+        k.shape[0] if packed else 0,
+        q.shape[-2] if q is not None else 0,
+        k.shape[-2],
+        SUPPORTED_HEAD_DIM,
+        k_pages.shape[0],
+        k_pages.shape[1],
+        page_table.shape[1],
+        2 * pairs,
+        1 if interleaved else 0,
+        1 if positions is not None and positions.dtype == torch.int64 else 0,
+        _DTYPES[k.dtype],
+        factor,
+        page_table.stride(0),
+        _position_strides(positions, packed) if positions is not None else (0, 0),
+        _token_strides(q) if q is not None else none,
+        _token_strides(k),
+        _token_strides(v),
+        _token_strides(q_out) if q is not None else none,
+        k_pages.stride()[:3],
+        v_pages.stride()[:3],
+    )
+    _call(lib.splitd_paged_append, params, k.device)
+    return q_out
+
+
+@torch.library.custom_op("splitd_flash_attn::paged_append", mutates_args=("k_pages", "v_pages"))
+def _paged_append_custom(
+    q: Optional[torch.Tensor],
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    page_table: torch.Tensor,
+    seqlens_k: torch.Tensor,
+    inv_freq: Optional[torch.Tensor],
+    positions: Optional[torch.Tensor],
+    cu_seqlens_q: Optional[torch.Tensor],
+    interleaved: bool,
+    factor: float,
+) -> torch.Tensor:
+    """The rotated q; an empty tensor if there is none."""
+    _check_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q)
+    out = _paged_append(
+        q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q, interleaved, factor
+    )
+    return k.new_empty((0,)) if out is None else out
+
+
+@torch.library.register_fake("splitd_flash_attn::paged_append")
+def _paged_append_fake(
+    q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q, interleaved, factor
+):
+    _check_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q)
+    return k.new_empty((0,) if q is None else q.shape)
+
+
+def split_paged_append_func(
+    q: Optional[torch.Tensor],
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    page_table: torch.Tensor,
+    seqlens_k: torch.Tensor,
+    inv_freq: Optional[torch.Tensor] = None,
+    positions: Optional[torch.Tensor] = None,
+    cu_seqlens_q: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+    factor: float = 1.0,
+):
+    """New tokens into a paged cache, in place, in one launch with the rotation of their queries and keys. Returns the
+    rotated q (None if q is None). Forward only.
+
+    Batched: q (B, S, Hq, 512), k and v (B, S, heads_kv, 512), S new tokens per sequence. Packed: (T, heads, 512) and
+    ``cu_seqlens_q`` int32 of B + 1 entries, any number of tokens per sequence (its values are checked as in
+    ``split_flash_attn_varlen_func``; ``cu_seqlens_validation(False)`` leaves that out). ``seqlens_k[b]`` is the length
+    of sequence b WITH its new tokens, which fill its last slots. Tokens whose slot would be negative are not stored
+    (length 0: a row that only pads the batch); two tokens must not share a slot.
+
+    ``inv_freq``, ``interleaved``, ``factor``: as in ``split_rotary_func``; without ``inv_freq`` nothing is rotated.
+    Positions are the slots, unless ``positions`` (one per token, int32 or int64) says otherwise, as it has to after an
+    eviction.
+    """
+    _check_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, k_pages, v_pages)):
+        raise NotImplementedError("SplitD paged append has no backward: call it under torch.no_grad() or detach its inputs")
+    interleaved, factor = bool(interleaved), float(factor)
+    args = (q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q)
+    if _traced(*args):
+        out = torch.ops.splitd_flash_attn.paged_append(*args, interleaved, factor)
+        return None if q is None else out
+    return _paged_append(*args, interleaved, factor)
+
+
+# ---------------------------------------------------------------------------
+# eviction
+# ---------------------------------------------------------------------------
+
+
+def _check_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent) -> None:
+    _check_cache(k_pages, v_pages, page_table, seqlens_k)
+    batch = seqlens_k.shape[0]
+    _check_weights(key_weights, batch, k_pages.device)
+    _check_table(new_page_table, "new_page_table", batch, k_pages.device)
+    for name, n in (("keep", keep), ("keep_first", keep_first), ("keep_recent", keep_recent)):
+        if isinstance(n, bool) or not isinstance(n, int):
+            raise TypeError(f"{name} must be an int, got {type(n).__name__}")
+        if n < 0:
+            raise ValueError(f"{name} must be non-negative, got {n}")
+    if keep < 1 or keep < keep_first + keep_recent:
+        raise ValueError(f"keep ({keep}) must be at least 1 and at least keep_first + keep_recent ({keep_first} + {keep_recent})")
+    if keep > 2**31 - 1:
+        raise ValueError(f"keep ({keep}) does not fit 32 bits")
+    if new_page_table.shape[1] * k_pages.shape[1] < keep:
+        raise ValueError(
+            f"new_page_table has {new_page_table.shape[1]} pages of {k_pages.shape[1]} slots per sequence, too few for {keep}"
+        )
+
+
+def _paged_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent):
+    _check_aligned(k_pages, v_pages)
+    device = k_pages.device
+    batch = seqlens_k.shape[0]
+    new_seqlens = torch.empty(batch, dtype=torch.int32, device=device)
+    kept = torch.empty((batch, keep), dtype=torch.int32, device=device)
+    new_weights = torch.empty((batch, keep), dtype=torch.float32, device=device)
+    if batch == 0:
+        return new_seqlens, kept, new_weights
+    page_table, new_page_table, seqlens_k = _unit_rows(page_table), _unit_rows(new_page_table), _unit_rows(seqlens_k)
+    lib = _capi.load_library()
+    params = _capi.SplitdEvictParams(
+        k_pages.data_ptr() or 256,  # see _paged_attn
+        v_pages.data_ptr() or 256,
+        page_table.data_ptr() or 256,
+        new_page_table.data_ptr(),
+        seqlens_k.data_ptr(),
+        key_weights.data_ptr() or 256,
+        new_seqlens.data_ptr(),
+        kept.data_ptr(),
+        new_weights.data_ptr(),
+        _status_flag(device).data_ptr(),
+        batch,
+        k_pages.shape[2],
+        SUPPORTED_HEAD_DIM,
+        k_pages.shape[0],
+        k_pages.shape[1],
+        page_table.shape[1],
+        new_page_table.shape[1],
+        key_weights.shape[1],
+        keep,
+        keep_first,
+        keep_recent,
+        page_table.stride(0),
+        new_page_table.stride(0),
+        key_weights.stride(0),
+        k_pages.stride()[:3],
+        v_pages.stride()[:3],
+    )
+    _call(lib.splitd_paged_evict, params, device)
+    return new_seqlens, kept, new_weights
+
+
+@torch.library.custom_op("splitd_flash_attn::paged_evict", mutates_args=("k_pages", "v_pages"))
+def _paged_evict_custom(
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    page_table: torch.Tensor,
+    seqlens_k: torch.Tensor,
+    key_weights: torch.Tensor,
+    new_page_table: torch.Tensor,
+    keep: int,
+    keep_first: int,
+    keep_recent: int,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    args = (k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
+    _check_evict(*args)
+    return _paged_evict(*args)
+
+
+@torch.library.register_fake("splitd_flash_attn::paged_evict")
+def _paged_evict_fake(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent):
+    _check_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
+    batch = seqlens_k.shape[0]
+    return seqlens_k.new_empty((batch,)), seqlens_k.new_empty((batch, keep)), key_weights.new_empty((batch, keep))
+
+
+def split_paged_evict_func(
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    page_table: torch.Tensor,
+    seqlens_k: torch.Tensor,
+    key_weights: torch.Tensor,
+    new_page_table: torch.Tensor,
+    keep: int,
+    keep_first: int = 0,
+    keep_recent: int = 0,
+):
+    """Shortens every sequence to at most ``keep`` slots: its first ``keep_first``, its last ``keep_recent``, and of the
+    others those with the largest ``key_weights`` (of equal ones the lower slot; NaN counts as the largest). The kept keys
+    and values are copied, in slot order, to the pages of ``new_page_table`` (B, new pages per sequence), which no
+    sequence may be using: pages are often shared between sequences, so none is changed in place. Sequences that are
+    short enough already are copied as they are; leave them out of the call to leave them alone.
+
+    Returns ``(new_seqlens, kept, new_weights)``: (B,) int32 lengths; (B, keep) int32 old slots, ascending, -1 behind
+    the last; (B, keep) float32 their weights, 0 behind the last, which go on being ``key_weights`` of the new cache.
+    Keys keep the rotation of the position they had, so tokens that follow need ``positions`` in
+    ``split_paged_append_func``.
+    """
+    args = (k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
+    _check_evict(*args)
+    if _traced(*args[:6]):
+        return torch.ops.splitd_flash_attn.paged_evict(*args)
+    return _paged_evict(*args)

@@ -85,7 +85,9 @@ typedef struct {
   /* device word, may be NULL. Every wait inside the kernels is bounded (4 s); a kernel that gives one up stores a
      positive code here with compare-and-swap against 0 and ends early, leaving its outputs incomplete:
      101 loads, 102 tensor-core issue, 103 softmax / epilogue, 104 peer CTA, 105 misaligned shared memory,
-     106 a packed sequence longer than max_seqlen_k. 0 = fine. Read it after synchronising; zero it to re-arm. */
+     106 a packed sequence longer than max_seqlen_k, 107 a page table names a page that the cache does not have,
+     108 a sequence is longer than its row of the page table (or of key_weights).
+     0 = fine. Read it after synchronising; zero it to re-arm. */
   int32_t* status_flag;
 
   /* reserved, must be NULL. (Builds made with -DSPLITD_PROFILE write per-role cycle counters of one CTA pair
@@ -210,6 +212,127 @@ int splitd_bwd(const splitd_params* p, void* stream);
 int splitd_bwd_static_scratch(const splitd_params* p, void* stream);
 size_t splitd_bwd_static_scratch_limit_rowstat(void);   /* 65536 floats   */
 size_t splitd_bwd_static_scratch_limit_workspace(void); /* 16 MiB         */
+
+/* ------------------------------------------------------------------------------------------------------------------
+ * Operators around a paged cache of keys and values, and rotary positions. No counterpart in the reference, which has
+ * no cache. The conventions above hold: device pointers of the caller, element strides with an innermost stride of 1,
+ * nothing allocated, nothing synchronised, work enqueued on `stream` of the current device.
+ *
+ * A cache is two tensors of pages (num_pages, page_size, heads_kv, 512). Slot j of sequence b is row j % page_size of
+ * page page_table[b * page_table_stride + j / page_size]. Page ids and lengths live on the device and are checked
+ * there: a row of a page that does not exist is neither read (it counts as zeros) nor written, a length beyond the
+ * table's row is cut to it, and both leave a code in *status_flag (107, 108). Entries of the table behind a sequence's
+ * last slot are never read. All rows are moved in pieces of 16 bytes: base addresses are 16-byte aligned and strides
+ * multiples of 8 elements.
+ * ------------------------------------------------------------------------------------------------------------------ */
+
+/* Attention of seqlen_q query tokens per sequence (one when decoding, a few when verifying drafted ones) over the
+ * cache. seqlens_k[b] counts the slots of sequence b with the new tokens in it: query i stands at slot
+ * seqlens_k[b] - seqlen_q + i, which is where causal and the window are measured from. Rows without a visible key get
+ * o = 0 and lse = -inf; slots that no query row of the sequence may see are not read at all. */
+typedef struct {
+  const void* q;       /* (B, Sq, Hq, 512) */
+  const void* k_pages; /* (num_pages, page_size, Hkv, 512) */
+  const void* v_pages;
+  void* o;                   /* like q; written */
+  float* lse;                /* (B, Hq, Sq) fp32, natural log; may be NULL */
+  float* key_weights;        /* (B, key_weights_len) fp32, may be NULL: [b, j] += sum over all query rows and heads of
+                                the softmax weight of slot j. Slots at or beyond key_weights_len are not counted */
+  const int32_t* page_table; /* (B, max_pages) */
+  const int32_t* seqlens_k;  /* (B) */
+  void* workspace;           /* splitd_paged_attn_workspace_bytes() bytes, 256-byte aligned; free again when the call's
+                                work has run. Calls that may overlap on the GPU need one each */
+  size_t workspace_bytes;
+  int32_t* status_flag; /* see splitd_params */
+  int32_t batch, seqlen_q, heads_q, heads_kv, head_dim;
+  int32_t num_pages, page_size, max_pages;
+  int32_t key_weights_len;
+  int32_t dtype, causal;
+  int32_t local, window_left, window_right; /* as in splitd_params */
+  float softmax_scale, softcap;
+  int64_t page_table_stride, key_weights_stride;
+  int64_t q_strides[3], o_strides[3];       /* batch, token, head */
+  int64_t k_strides[3], v_strides[3];       /* page, row of the page, head */
+} splitd_paged_params;
+
+int splitd_paged_attn(const splitd_paged_params* p, void* stream);
+size_t splitd_paged_attn_workspace_bytes(const splitd_paged_params* p);
+
+/* Rotary positions on the first rotary_dim dimensions of every query and key head: pair i of a token at position t is
+ * turned by t * inv_freq[i] and scaled by factor. A pair is dimensions (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with
+ * interleaved. backward = 1 turns the other way: the gradients of the inputs from those of the outputs. q or k may be
+ * NULL. Packed tokens: batch = 1, seqlen = tokens. */
+typedef struct {
+  const void* q; /* (B, S, Hq, 512) */
+  const void* k; /* (B, S, Hkv, 512) */
+  void* q_out;
+  void* k_out;
+  const void* positions;  /* (B, S) int32, or int64 with positions_64bit */
+  const double* inv_freq; /* rotary_dim / 2 */
+  int32_t batch, seqlen, heads_q, heads_kv, head_dim;
+  int32_t rotary_dim, interleaved, backward, positions_64bit, dtype;
+  float factor;
+  int64_t position_strides[2];                 /* batch, token; 0 for positions that all sequences share */
+  int64_t q_strides[3], k_strides[3];          /* batch, token, head */
+  int64_t q_out_strides[3], k_out_strides[3];
+} splitd_rotary_params;
+
+int splitd_rotary(const splitd_rotary_params* p, void* stream);
+
+/* New tokens into the cache: key and value of token t of sequence b go to slot seqlens_k[b] - n_b + t, where n_b is the
+ * number of its new tokens and seqlens_k[b] its length with them; keys are turned on the way as splitd_rotary does
+ * (inv_freq NULL: not at all), at the slot or, if given, at positions. q, if given, is turned too and written to q_out.
+ * Tokens whose slot is negative (a sequence of length 0 in a padded batch) or that lie behind the last sequence are
+ * not stored. Batched: (B, S, heads, 512) and cu_seqlens NULL; packed: (total_tokens, heads, 512) and cu_seqlens. */
+typedef struct {
+  const void* q; /* may be NULL */
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_pages;
+  void* v_pages;
+  const int32_t* page_table;
+  const int32_t* seqlens_k;
+  const int32_t* cu_seqlens; /* B + 1 entries, or NULL */
+  const void* positions;     /* per token, or NULL */
+  const double* inv_freq;    /* rotary_dim / 2, or NULL */
+  int32_t* status_flag;
+  int32_t batch, seqlen, total_tokens, heads_q, heads_kv, head_dim;
+  int32_t num_pages, page_size, max_pages;
+  int32_t rotary_dim, interleaved, positions_64bit, dtype;
+  float factor;
+  int64_t page_table_stride;
+  int64_t position_strides[2];
+  int64_t q_strides[3], k_strides[3], v_strides[3], q_out_strides[3]; /* batch, token, head; packed ignores [0] */
+  int64_t k_page_strides[3], v_page_strides[3];                       /* page, row of the page, head */
+} splitd_append_params;
+
+int splitd_paged_append(const splitd_append_params* p, void* stream);
+
+/* Eviction: of the n = seqlens_k[b] slots of a sequence keep min(n, keep), the first keep_first, the last keep_recent
+ * and of the others those with the largest key_weights (equal weights: the lower slot; NaN counts as the largest), and
+ * copy their keys and values, in slot order, to the pages of new_page_table, which no sequence of the call may be
+ * using. kept[b] gets the old slots (-1 behind the last), new_weights[b] their weights (0 behind the last),
+ * new_seqlens[b] their number. A sequence longer than key_weights_len is cut to it (status 108). */
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  const int32_t* page_table;     /* (B, max_pages) */
+  const int32_t* new_page_table; /* (B, new_max_pages), new_max_pages * page_size >= keep */
+  const int32_t* seqlens_k;
+  const float* key_weights; /* (B, key_weights_len) */
+  int32_t* new_seqlens;     /* (B) */
+  int32_t* kept;            /* (B, keep) contiguous */
+  float* new_weights;       /* (B, keep) contiguous */
+  int32_t* status_flag;
+  int32_t batch, heads_kv, head_dim;
+  int32_t num_pages, page_size, max_pages, new_max_pages;
+  int32_t key_weights_len, keep, keep_first, keep_recent;
+  int64_t page_table_stride, new_page_table_stride, key_weights_stride;
+  int64_t k_strides[3], v_strides[3]; /* page, row of the page, head */
+} splitd_evict_params;
+
+int splitd_paged_evict(const splitd_evict_params* p, void* stream);
 
 /* Test aid, on no product path: one small CTA waits with the kernels' bounded wait on a barrier that nobody
  * arrives on, for limit_us microseconds (1 .. 100000), then stores code 104 in *status_flag (device memory)
