@@ -36,7 +36,9 @@ constexpr int kStages = 6;
 constexpr int kPitch = kRowBytes + 16;         // ldmatrix reads 8 rows at once: 16 bytes of padding spread them over the banks
 constexpr int kStageBytes = kTile * kPitch;
 constexpr int kConsumers = 256;                // threads of the eight warps that compute
-constexpr int kThreads = kConsumers + 32;
+constexpr int kProducers = 4;                  // producer warps: each asks for a quarter of a tile's rows
+constexpr int kRowsPerProducer = kTile / kProducers;
+constexpr int kThreads = kConsumers + 32 * kProducers;
 constexpr int kPartPitch = 36;                 // floats per row of the partial scores (32 keys + padding)
 constexpr int kPPitch = 20;                    // 32-bit words per row of P (32 keys x 2 bytes + padding)
 constexpr int kMaxRows = 32;                   // rows of a row block
@@ -157,8 +159,10 @@ struct Ring {
 };
 
 template <int kNB>
-__device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem, Ring r, volatile int* abort_flag, int lane) {
+__device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem, Ring r, volatile int* abort_flag, int pw, int lane) {
   using L = Layout<kNB>;
+  const int my_row = pw * kRowsPerProducer + lane % kRowsPerProducer;  // row of a tile; lanes beyond kRowsPerProducer are idle
+  const bool active = lane < kRowsPerProducer;
   Desc* descs = reinterpret_cast<Desc*>(smem + L::kOffDesc);
   const uint32_t ring0 = smem_u32(smem);
   int used = 0;  // stages handed out
@@ -215,19 +219,20 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
       if (!acquire()) break;
       {
         const uint32_t bar = r.full + 8 * r.stage;
-        if (lane == 0) {
+        const uint32_t rows = __popc(__ballot_sync(0xffffffffu, active && my_row < n_rows));
+        if (lane == 0 && pw == 0) {
           Desc d;
           d.b = b, d.head = head, d.row0 = row0, d.n_tiles = n;
           d.len = len, d.first_key = lo + tile0 * kTile;
           d.slot = n == n_tiles ? -1 : (tile0 > 0 ? 0 : 1);
           d.pad = 0;
           descs[r.stage] = d;
-          mbar_arrive_expect_tx(bar, n_rows * kRowBytes);
         }
+        if (lane == 0) mbar_arrive_expect_tx(bar, rows * kRowBytes);
         __syncwarp();
-        if (lane < n_rows) {
-          const int i = (row0 + lane) / p.group, g = (row0 + lane) - i * p.group;
-          bulk_load(ring0 + r.stage * kStageBytes + lane * kPitch, p.q + b * p.q_sb + i * p.q_ss + (head * p.group + g) * p.q_sh,
+        if (active && my_row < n_rows) {
+          const int i = (row0 + my_row) / p.group, g = (row0 + my_row) - i * p.group;
+          bulk_load(ring0 + r.stage * kStageBytes + my_row * kPitch, p.q + b * p.q_sb + i * p.q_ss + (head * p.group + g) * p.q_sh,
                     kRowBytes, bar);
         }
         r.next(), ++used;
@@ -241,14 +246,14 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
           page = page_of(p.map, b, entry);
         }
       };
-      int slot = lo + tile0 * kTile + lane, page, row;
+      int slot = lo + tile0 * kTile + my_row, page, row;
       lookup(slot, page, row);
       for (int i = 0; i < n && ok; ++i) {
         int next_page = -1, next_row = 0;
         if (i + 1 < n) lookup(slot + kTile, next_page, next_row);
         const bool inside = slot < len;
-        const bool have = inside && page_ok(p.map, page);
-        if (inside && !have && p.status) atomicCAS(p.status, 0, ST_BAD_PAGE);
+        const bool have = inside && active && page_ok(p.map, page);
+        if (inside && active && !have && p.status) atomicCAS(p.status, 0, ST_BAD_PAGE);
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, have)) * kRowBytes;
         const uint16_t* src[2] = {p.k + page * p.k_sp + row * p.k_ss + head * p.k_sh,
                                   p.v + page * p.v_sp + row * p.v_ss + head * p.v_sh};
@@ -256,8 +261,8 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
         for (int kv = 0; kv < 2; ++kv) {
           if (!acquire()) break;
           const uint32_t bar = r.full + 8 * r.stage;
-          const uint32_t dst = ring0 + r.stage * kStageBytes + lane * kPitch;
-          if (!have) {  // a row that is not there counts as zeros: 0 * (what lay there) could be NaN
+          const uint32_t dst = ring0 + r.stage * kStageBytes + my_row * kPitch;
+          if (active && !have) {  // a row that is not there counts as zeros: 0 * (what lay there) could be NaN
             for (int c = 0; c < kRowBytes; c += 16) st_shared_v4(dst + c, 0, 0, 0, 0);
             fence_proxy_async_smem();
           }
@@ -283,7 +288,7 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
   }
   if (acquire()) {
     if (lane == 0) {
-      descs[r.stage].n_tiles = 0;
+      if (pw == 0) descs[r.stage].n_tiles = 0;
       mbar_arrive(r.full + 8 * r.stage);
     }
   } else {
@@ -534,15 +539,15 @@ __global__ void __launch_bounds__(kThreads, 1) splitd_paged_attn_kernel(const __
   r.empty = r.full + 8 * kStages;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(r.full + 8 * i, 1);
+      mbar_init(r.full + 8 * i, kProducers);
       mbar_init(r.empty + 8 * i, kConsumers / 32);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
   __syncthreads();
-  if (warp == kConsumers / 32)
-    producer<kNB>(p, smem, r, abort_flag, lane);
+  if (warp >= kConsumers / 32)
+    producer<kNB>(p, smem, r, abort_flag, warp - kConsumers / 32, lane);
   else
     consumer<kFp16, kNB>(p, smem, r, abort_flag, warp, lane);
 }
