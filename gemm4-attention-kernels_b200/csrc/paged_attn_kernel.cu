@@ -32,7 +32,6 @@ namespace sd {
 
 namespace pa {
 constexpr int kTile = 32;                      // keys per tile = rows per ring stage
-constexpr int kStages = 6;
 constexpr int kPitch = kRowBytes + 16;         // ldmatrix reads 8 rows at once: 16 bytes of padding spread them over the banks
 constexpr int kStageBytes = kTile * kPitch;
 constexpr int kConsumers = 256;                // threads of the eight warps that compute
@@ -42,6 +41,13 @@ constexpr int kThreads = kConsumers + 32 * kProducers;
 constexpr int kPartPitch = 36;                 // floats per row of the partial scores (32 keys + padding)
 constexpr int kPPitch = 20;                    // 32-bit words per row of P (32 keys x 2 bytes + padding)
 constexpr int kMaxRows = 32;                   // rows of a row block
+
+// From 17 rows on a consumer thread needs more than the 168 registers that 384 threads can have each, so the producers
+// give up some of theirs (4 tokens, 32 rows: 305 us with spills, 159 us with the split; with 8 rows the split costs 1 %).
+// The launch checks that the block comes with at least as many as the two shares together.
+template <int kNB>
+constexpr bool kSplitRegs = kNB >= 3;
+constexpr int kProducerRegs = 56, kConsumerRegs = 216;
 
 struct Desc {  // what the producer tells the others about a stretch of tiles
   int b, head, row0, n_tiles;  // n_tiles == 0: no more work
@@ -53,11 +59,17 @@ struct Desc {  // what the producer tells the others about a stretch of tiles
 template <int kNB>
 struct Layout {
   static constexpr int kRows = 8 * kNB;
+  // two of each of these: one tile's are read while the next one's are written
+  static constexpr int kPartFloats = 4 * kRows * kPartPitch;
+  static constexpr int kPWords = kRows * kPPitch;  // of each half of P
+  // as many stages as fit beside them; four in flight are enough to cover the latency of HBM
+  static constexpr int kStages = kNB <= 2 ? 6 : 5;
   static constexpr int kOffPart = kStages * kStageBytes;
-  static constexpr int kOffP = kOffPart + 4 * kRows * kPartPitch * 4;
-  static constexpr int kOffCorr = kOffP + 2 * kRows * kPPitch * 4;
-  static constexpr int kOffStat = kOffCorr + kRows * 4;
-  static constexpr int kOffDesc = kOffStat + kRows * 8;
+  static constexpr int kOffP = kOffPart + 2 * kPartFloats * 4;
+  static constexpr int kOffCorr = kOffP + 2 * 2 * kPWords * 4;
+  static constexpr int kOffStat = kOffCorr + 2 * kRows * 4;
+  static constexpr int kOffBounds = kOffStat + kRows * 8;
+  static constexpr int kOffDesc = kOffBounds + kRows * 8;
   static constexpr int kOffBar = kOffDesc + kStages * static_cast<int>(sizeof(Desc));
   static constexpr int kOffAbort = kOffBar + 2 * kStages * 8;
   static constexpr int kBytes = kOffAbort + 16;
@@ -149,6 +161,14 @@ __device__ __forceinline__ void split16(float p, uint16_t& hi, uint16_t& lo) {
   }
 }
 
+// largest value of the warp in all lanes; NaN are passed over
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int kStages>
 struct Ring {
   uint32_t full, empty;  // barrier arrays
   int stage = 0;
@@ -159,7 +179,8 @@ struct Ring {
 };
 
 template <int kNB>
-__device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem, Ring r, volatile int* abort_flag, int pw, int lane) {
+__device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem, Ring<Layout<kNB>::kStages> r, volatile int* abort_flag, int pw,
+                                         int lane) {
   using L = Layout<kNB>;
   const int my_row = pw * kRowsPerProducer + lane % kRowsPerProducer;  // row of a tile; lanes beyond kRowsPerProducer are idle
   const bool active = lane < kRowsPerProducer;
@@ -172,7 +193,9 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
     ok = __all_sync(0xffffffffu, ok);
     return ok;
   };
-  const Line line = make_line(p, tiles_before(p, p.batch, lane));
+  // up to 32 sequences: their lengths are read once
+  const int len0 = lane < p.batch ? seq_len(p, lane) : 0;
+  const Line line = make_line(p, p.batch <= 32 ? warp_sum(seq_tiles(p, len0)) * (p.heads_kv * p.row_blocks) : tiles_before(p, p.batch, lane));
   const int cta = blockIdx.x;
   if (cta < line.ctas) {
     long long t = line.begin(cta);
@@ -182,7 +205,7 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
     long long base = 0;
     int b = 0, len = 0, n_tiles = 0;
     for (int b0 = 0;; b0 += 32) {
-      const int my_len = b0 + lane < p.batch ? seq_len(p, b0 + lane) : 0;
+      const int my_len = b0 == 0 ? len0 : b0 + lane < p.batch ? seq_len(p, b0 + lane) : 0;
       const int mine = seq_tiles(p, my_len);
       long long incl = static_cast<long long>(mine) * units;
 #pragma unroll
@@ -248,30 +271,32 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
       };
       int slot = lo + tile0 * kTile + my_row, page, row;
       lookup(slot, page, row);
-      for (int i = 0; i < n && ok; ++i) {
+      const uint16_t* v_src = nullptr;
+      bool v_have = false;
+      auto ask = [&](const uint16_t* src, bool have) {
+        if (!acquire()) return;
+        const uint32_t bar = r.full + 8 * r.stage;
+        const uint32_t dst = ring0 + r.stage * kStageBytes + my_row * kPitch;
+        if (active && !have) {  // a row that is not there counts as zeros: 0 * (what lay there) could be NaN
+          for (int c = 0; c < kRowBytes; c += 16) st_shared_v4(dst + c, 0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, have)) * kRowBytes;
+        if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+        __syncwarp();
+        if (have) bulk_load(dst, src, kRowBytes, bar);
+        r.next(), ++used;
+      };
+      // in the order of use: K(0), K(1), V(0), K(2), V(1), ..., K(n - 1), V(n - 2), V(n - 1)
+      for (int i = 0; i <= n && ok; ++i) {
         int next_page = -1, next_row = 0;
         if (i + 1 < n) lookup(slot + kTile, next_page, next_row);
-        const bool inside = slot < len;
-        const bool have = inside && active && page_ok(p.map, page);
-        if (inside && active && !have && p.status) atomicCAS(p.status, 0, ST_BAD_PAGE);
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, have)) * kRowBytes;
-        const uint16_t* src[2] = {p.k + page * p.k_sp + row * p.k_ss + head * p.k_sh,
-                                  p.v + page * p.v_sp + row * p.v_ss + head * p.v_sh};
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (!acquire()) break;
-          const uint32_t bar = r.full + 8 * r.stage;
-          const uint32_t dst = ring0 + r.stage * kStageBytes + my_row * kPitch;
-          if (active && !have) {  // a row that is not there counts as zeros: 0 * (what lay there) could be NaN
-            for (int c = 0; c < kRowBytes; c += 16) st_shared_v4(dst + c, 0, 0, 0, 0);
-            fence_proxy_async_smem();
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
-          __syncwarp();
-          if (have) bulk_load(dst, src[kv], kRowBytes, bar);
-          r.next(), ++used;
-        }
+        const bool inside = active && i < n && slot < len;
+        const bool have = inside && page_ok(p.map, page);
+        if (inside && !have && p.status) atomicCAS(p.status, 0, ST_BAD_PAGE);
+        if (i < n) ask(p.k + page * p.k_sp + row * p.k_ss + head * p.k_sh, have);
+        if (i > 0) ask(v_src, v_have);
+        v_src = p.v + page * p.v_sp + row * p.v_ss + head * p.v_sh, v_have = have;
         slot += kTile, page = next_page, row = next_row;
       }
       t += n;
@@ -293,9 +318,9 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
     }
   } else {
     // a wait was given up: let the copies in flight land before the block ends
-    for (int i = 0; i < kStages && i < used; ++i) {
+    for (int i = 0; i < L::kStages && i < used; ++i) {
       r.phase ^= r.stage == 0;
-      r.stage = r.stage == 0 ? kStages - 1 : r.stage - 1;
+      r.stage = r.stage == 0 ? L::kStages - 1 : r.stage - 1;
       volatile int never = 0;
       mbar_wait_limit(r.full + 8 * r.stage, r.phase, &never, nullptr, 0, 1000ull * 1000ull * 1000ull);
     }
@@ -303,18 +328,16 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
 }
 
 template <bool kFp16, int kNB>
-__device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem, Ring r, volatile int* abort_flag, int warp,
-                                         int lane) {
+__device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem, Ring<Layout<kNB>::kStages> r,
+                                         volatile int* abort_flag, int warp, int lane) {
   using L = Layout<kNB>;
   constexpr int kRows = L::kRows;
   const Desc* descs = reinterpret_cast<const Desc*>(smem + L::kOffDesc);
-  float* part = reinterpret_cast<float*>(smem + L::kOffPart);
-  uint16_t* p_hi = reinterpret_cast<uint16_t*>(smem + L::kOffP);
-  uint16_t* p_lo = p_hi + kRows * kPPitch * 2;
-  const uint32_t* pw_hi = reinterpret_cast<const uint32_t*>(p_hi);
-  const uint32_t* pw_lo = reinterpret_cast<const uint32_t*>(p_lo);
-  float* corr = reinterpret_cast<float*>(smem + L::kOffCorr);
+  float* part0 = reinterpret_cast<float*>(smem + L::kOffPart);
+  uint32_t* p0 = reinterpret_cast<uint32_t*>(smem + L::kOffP);
+  float* corr0 = reinterpret_cast<float*>(smem + L::kOffCorr);
   float2* stat = reinterpret_cast<float2*>(smem + L::kOffStat);
+  int2* bounds = reinterpret_cast<int2*>(smem + L::kOffBounds);
   const uint32_t ring0 = smem_u32(smem);
   const int key_half = warp & 1, d_quarter = warp >> 1;
   const int frag_row = lane >> 2, frag_col = (lane & 3) * 2;
@@ -367,116 +390,152 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[mt][nb][e] = 0.f;
     float m_row[kNB], l_row[kNB];
-    int key_lo[kNB], key_hi[kNB];  // keys [key_lo, key_hi) are visible to the rows whose softmax this warp does
 #pragma unroll
     for (int k = 0; k < kNB; ++k) {
       m_row[k] = -INFINITY, l_row[k] = 0.f;
+      // keys [x, y) are visible to the row; only this warp reads its rows' bounds
       const int row = d.row0 + warp + 8 * k;
-      if (warp + 8 * k >= p.rows_per_block || row >= p.rows) {
-        key_lo[k] = 0, key_hi[k] = 0;
-      } else {
+      int2 vis = make_int2(0, 0);
+      if (warp + 8 * k < p.rows_per_block && row < p.rows) {
         const long long diag = static_cast<long long>(row / p.group) + d.len - p.sq;
-        key_lo[k] = p.win_left < 0 ? 0 : static_cast<int>(max(0ll, diag - p.win_left));
-        key_hi[k] = p.win_right < 0 ? d.len : static_cast<int>(max(0ll, min(static_cast<long long>(d.len), diag + p.win_right + 1)));
+        vis.x = p.win_left < 0 ? 0 : static_cast<int>(max(0ll, diag - p.win_left));
+        vis.y = p.win_right < 0 ? d.len : static_cast<int>(max(0ll, min(static_cast<long long>(d.len), diag + p.win_right + 1)));
       }
+      if (lane == 0) bounds[warp + 8 * k] = vis;
     }
-    for (int tile = 0; tile < d.n_tiles; ++tile) {
-      // ---- partial scores: 16 keys x rows over a quarter of the head dimension
-      wait_full();
-      float s[kNB][4];
+    __syncwarp();
+
+    // partial scores of the tile in the ring's next stage: 16 keys x rows over a quarter of the head dimension
+    float s[kNB][4];
+    auto scores = [&]() {
 #pragma unroll
       for (int nb = 0; nb < kNB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
-      {
-        const uint32_t base =
-            ring0 + r.stage * kStageBytes + (key_half * 16 + (lane & 15)) * kPitch + d_quarter * 256 + (lane >> 4) * 16;
+      wait_full();
+      const uint32_t base =
+          ring0 + r.stage * kStageBytes + (key_half * 16 + (lane & 15)) * kPitch + d_quarter * 256 + (lane >> 4) * 16;
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          uint32_t a[4];
-          ldmatrix_x4(base + ks * 32, a);
+      for (int ks = 0; ks < 8; ++ks) {
+        uint32_t a[4];
+        ldmatrix_x4(base + ks * 32, a);
 #pragma unroll
-          for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(s[nb], a, qf[ks][nb][0], qf[ks][nb][1]);
-        }
+        for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(s[nb], a, qf[ks][nb][0], qf[ks][nb][1]);
       }
       release();
+    };
+    auto put_scores = [&](int buf) {
+      float* part = part0 + buf * L::kPartFloats;
 #pragma unroll
       for (int nb = 0; nb < kNB; ++nb) {
         float* dst = part + (d_quarter * kRows + nb * 8 + frag_col) * kPartPitch + key_half * 16 + frag_row;
         dst[0] = s[nb][0], dst[kPartPitch] = s[nb][1], dst[8] = s[nb][2], dst[kPartPitch + 8] = s[nb][3];
       }
-      sync();
-      // ---- softmax: one row per warp (and n tile), one key per lane
+    };
+    // softmax: one row per warp (and n tile), one key per lane
+    auto softmax = [&](int tile, int buf) {
       const int key = d.first_key + tile * kTile + lane;
+      uint16_t* p_hi = reinterpret_cast<uint16_t*>(p0 + buf * 2 * L::kPWords);
+      uint16_t* p_lo = p_hi + 2 * L::kPWords;
+      // step by step over all rows, so that their latencies overlap
+      float x[kNB], top[kNB];
+#pragma unroll
+      for (int k = 0; k < kNB; ++k) {
+        const float* src = part0 + buf * L::kPartFloats + (warp + 8 * k) * kPartPitch + lane;
+        x[k] = (src[0] + src[kRows * kPartPitch]) + (src[2 * kRows * kPartPitch] + src[3 * kRows * kPartPitch]);
+      }
+      if (p.softcap > 0.f) {
+#pragma unroll
+        for (int k = 0; k < kNB; ++k) x[k] = cap_out * tanhf(x[k] * cap_in);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kNB; ++k) x[k] *= scale_log2;
+      }
+#pragma unroll
+      for (int k = 0; k < kNB; ++k) {
+        const int2 vis = bounds[warp + 8 * k];
+        if (key < vis.x || key >= vis.y) x[k] = -INFINITY;
+        top[k] = warp_max(x[k]);
+      }
+      if (p.scores) {
+#pragma unroll
+        for (int k = 0; k < kNB; ++k)
+          if (key < d.len && key < p.weights_len && bounds[warp + 8 * k].y > 0)
+            p.scores[(static_cast<int64_t>(d.b) * p.heads_kv * p.rows + d.head * p.rows + d.row0 + warp + 8 * k) * p.weights_len + key] = x[k];
+      }
 #pragma unroll
       for (int k = 0; k < kNB; ++k) {
         const int row = warp + 8 * k;
-        const float* src = part + row * kPartPitch + lane;
-        float x = (src[0] + src[kRows * kPartPitch]) + (src[2 * kRows * kPartPitch] + src[3 * kRows * kPartPitch]);
-        x = p.softcap > 0.f ? cap_out * tanhf(x * cap_in) : x * scale_log2;
-        if (key < key_lo[k] || key >= key_hi[k]) x = -INFINITY;
-        if (p.scores && key < d.len && key < p.weights_len && key_hi[k] > 0)
-          p.scores[(static_cast<int64_t>(d.b) * p.heads_kv * p.rows + d.head * p.rows + d.row0 + row) * p.weights_len + key] = x;
-        float top = x;
-#pragma unroll
-        for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-        const float m_new = fmaxf(m_row[k], top);
-        float c = 1.f, e = 0.f;
-        if (m_new != -INFINITY) {
-          c = ex2(m_row[k] - m_new);
-          e = ex2(x - m_new);
-        } else if (x != x) {
-          e = x;  // every visible score is NaN: the row has to become NaN too
-        }
+        const float m_new = fmaxf(m_row[k], top[k]);
+        // a row that has seen no key yet: any finite reference gives p = 0 (and NaN for scores that are NaN)
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        const float c = ex2(m_row[k] - ref), e = ex2(x[k] - ref);
         m_row[k] = m_new;
         l_row[k] = l_row[k] * c + e;
         uint16_t hi, lo;
         split16<kFp16>(e, hi, lo);
         p_hi[row * kPPitch * 2 + lane] = hi, p_lo[row * kPPitch * 2 + lane] = lo;
-        if (lane == 0) corr[row] = c;
+        if (lane == 0) corr0[buf * kRows + row] = c;
       }
-      sync();
-      // ---- O^T += V^T P^T, 64 columns of the head dimension
+    };
+    // O^T += V^T P^T with the tile in the ring's next stage, 64 columns of the head dimension
+    auto values = [&](int buf) {
       wait_full();
-      {
-        float cf[kNB][2];
-        bool any = false;
+      const float* corr = corr0 + buf * kRows;
+      const uint32_t* pw_hi = p0 + buf * 2 * L::kPWords;
+      const uint32_t* pw_lo = pw_hi + L::kPWords;
+      float cf[kNB][2];
+      bool any = false;
 #pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          cf[nb][0] = corr[nb * 8 + frag_col], cf[nb][1] = corr[nb * 8 + frag_col + 1];
-          any |= cf[nb][0] != 1.f || cf[nb][1] != 1.f;
-        }
-        if (__any_sync(0xffffffffu, any)) {
+      for (int nb = 0; nb < kNB; ++nb) {
+        cf[nb][0] = corr[nb * 8 + frag_col], cf[nb][1] = corr[nb * 8 + frag_col + 1];
+        any |= cf[nb][0] != 1.f || cf[nb][1] != 1.f;
+      }
+      if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
-          for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-            for (int nb = 0; nb < kNB; ++nb) {
-              o[mt][nb][0] *= cf[nb][0], o[mt][nb][1] *= cf[nb][1];
-              o[mt][nb][2] *= cf[nb][0], o[mt][nb][3] *= cf[nb][1];
-            }
-        }
-        const uint32_t base = ring0 + r.stage * kStageBytes + ((lane & 7) + (lane >> 4) * 8) * kPitch + warp * 128 + ((lane >> 3) & 1) * 16;
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-          uint32_t bh[kNB][2], bl[kNB][2];
+        for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
           for (int nb = 0; nb < kNB; ++nb) {
-            const int at = (nb * 8 + frag_row) * kPPitch + ks * 8 + (lane & 3);
-            bh[nb][0] = pw_hi[at], bh[nb][1] = pw_hi[at + 4];
-            bl[nb][0] = pw_lo[at], bl[nb][1] = pw_lo[at + 4];
+            o[mt][nb][0] *= cf[nb][0], o[mt][nb][1] *= cf[nb][1];
+            o[mt][nb][2] *= cf[nb][0], o[mt][nb][3] *= cf[nb][1];
           }
+      }
+      const uint32_t base =
+          ring0 + r.stage * kStageBytes + ((lane & 7) + (lane >> 4) * 8) * kPitch + warp * 128 + ((lane >> 3) & 1) * 16;
 #pragma unroll
-          for (int mt = 0; mt < 4; ++mt) {
-            uint32_t a[4];
-            ldmatrix_x4_trans(base + ks * 16 * kPitch + mt * 32, a);
+      for (int ks = 0; ks < 2; ++ks) {
+        uint32_t bh[kNB][2], bl[kNB][2];
 #pragma unroll
-            for (int nb = 0; nb < kNB; ++nb) {
-              mma_16816<kFp16>(o[mt][nb], a, bh[nb][0], bh[nb][1]);
-              mma_16816<kFp16>(o[mt][nb], a, bl[nb][0], bl[nb][1]);
-            }
-          }
+        for (int nb = 0; nb < kNB; ++nb) {
+          const int at = (nb * 8 + frag_row) * kPPitch + ks * 8 + (lane & 3);
+          bh[nb][0] = pw_hi[at], bh[nb][1] = pw_hi[at + 4];
+          bl[nb][0] = pw_lo[at], bl[nb][1] = pw_lo[at + 4];
+        }
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          uint32_t a[4];
+          ldmatrix_x4_trans(base + ks * 16 * kPitch + mt * 32, a);
+#pragma unroll
+          for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(o[mt][nb], a, bh[nb][0], bh[nb][1]);
+#pragma unroll
+          for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(o[mt][nb], a, bl[nb][0], bl[nb][1]);
         }
       }
       release();
+    };
+    // One barrier per tile. Between two of them the warps have three independent things to do: the values of the tile
+    // before, the scores of the tile behind, and the softmax of this one.
+    scores();
+    put_scores(0);
+    sync();
+    for (int tile = 0; tile < d.n_tiles; ++tile) {
+      const int buf = tile & 1;
+      if (tile > 0) values(buf ^ 1);
+      const bool more = tile + 1 < d.n_tiles;
+      if (more) scores();
+      softmax(tile, buf);
+      if (more) put_scores(buf ^ 1);
+      sync();
     }
+    values((d.n_tiles - 1) & 1);
     // ---- the stretch is done
 #pragma unroll
     for (int k = 0; k < kNB; ++k) {
@@ -534,11 +593,11 @@ __global__ void __launch_bounds__(kThreads, 1) splitd_paged_attn_kernel(const __
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffAbort);
-  Ring r;
+  Ring<L::kStages> r;
   r.full = smem_u32(smem + L::kOffBar);
-  r.empty = r.full + 8 * kStages;
+  r.empty = r.full + 8 * L::kStages;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < L::kStages; ++i) {
       mbar_init(r.full + 8 * i, kProducers);
       mbar_init(r.empty + 8 * i, kConsumers / 32);
     }
@@ -546,20 +605,23 @@ __global__ void __launch_bounds__(kThreads, 1) splitd_paged_attn_kernel(const __
     fence_mbar_init();
   }
   __syncthreads();
-  if (warp >= kConsumers / 32)
+  if (warp >= kConsumers / 32) {
+    if constexpr (kSplitRegs<kNB>) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
     producer<kNB>(p, smem, r, abort_flag, warp - kConsumers / 32, lane);
-  else
+  } else {
+    if constexpr (kSplitRegs<kNB>) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
     consumer<kFp16, kNB>(p, smem, r, abort_flag, warp, lane);
+  }
 }
 
-constexpr int kJoinThreads = 512;
-constexpr int kJoinGroups = kJoinThreads / 128;
-
 // One block per output row: adds up the partial results of the CTAs that share the row's unit, or writes the row of a
-// sequence without keys. Rows whose unit lay inside one CTA are finished already.
-template <bool kFp16>
-__global__ void __launch_bounds__(kJoinThreads) splitd_paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
-  __shared__ float acc[kJoinGroups][kHeadDim];
+// sequence without keys. Rows whose unit lay inside one CTA are finished already. kGroups groups of kCols / 4 threads, 4
+// columns each; group g takes every kGroups-th partial result; blockIdx.z counts slices of kCols columns.
+template <bool kFp16, int kGroups, int kCols>
+__global__ void __launch_bounds__(kGroups * kCols / 4) splitd_paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
+  constexpr int kPer = kCols / 4;  // threads of a group
+  __shared__ float4 acc[kGroups][kGroups > 1 ? kPer : 1];
+  const int col0 = blockIdx.z * kCols;
   __shared__ long long span[3];  // line total, first tile of this sequence, tiles of a unit of it
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -569,77 +631,85 @@ __global__ void __launch_bounds__(kJoinThreads) splitd_paged_join_kernel(const _
   const int units = p.heads_kv * p.row_blocks;
   if (hr == 0 && tid == 0 && __ldg(p.seqlens + b) > page_capacity(p.map) && p.status) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
   if (warp == 0) {
-    const long long before = tiles_before(p, b, lane);
-    long long after = 0;
-    for (int i = b + lane; i < p.batch; i += 32) after += seq_tiles(p, seq_len(p, i));
-    after = warp_sum(after) * units;
-    if (lane == 0) {
-      span[0] = before + after;
-      span[1] = before;
-      span[2] = seq_tiles(p, seq_len(p, b));
+    long long before = 0, after = 0;
+    int mine = 0;
+    for (int i = lane; i < p.batch; i += 32) {
+      const int t = seq_tiles(p, seq_len(p, i));
+      if (i < b) before += t; else after += t;
+      if (i == b) mine = t;
     }
+    before = warp_sum(before) * units, after = warp_sum(after) * units;
+    mine = __shfl_sync(0xffffffffu, mine, b & 31);
+    if (lane == 0) span[0] = before + after, span[1] = before, span[2] = mine;
   }
   __syncthreads();
-  pdl_wait();
   const int n_tiles = static_cast<int>(span[2]);
   const int i = unit_row / p.group, g = unit_row - i * p.group;
   const int hq = head * p.group + g;
   uint16_t* out = p.o + b * p.o_sb + i * p.o_ss + hq * p.o_sh;
   const int64_t lse_at = (static_cast<int64_t>(b) * p.heads_q + hq) * p.sq + i;
   const int64_t lse2_at = static_cast<int64_t>(b) * p.heads_kv * p.rows + hr;
+  int c0 = 0, c1 = -1;
+  if (n_tiles > 0) {
+    const Line line = make_line(p, span[0]);
+    const long long t0 = span[1] + static_cast<long long>(head * p.row_blocks + rb) * n_tiles;
+    c0 = line.owner(t0), c1 = line.owner(t0 + n_tiles - 1);
+  }
+  pdl_wait();
   if (n_tiles == 0) {
-    for (int c = tid; c < kHeadDim; c += kJoinThreads) out[c] = 0;
-    if (tid == 0) {
+    if (tid < kCols / 8) *reinterpret_cast<uint4*>(out + col0 + tid * 8) = make_uint4(0, 0, 0, 0);
+    if (tid == 0 && col0 == 0) {
       if (p.lse) p.lse[lse_at] = -INFINITY;
       if (p.lse2) p.lse2[lse2_at] = -INFINITY;
     }
     return;
   }
-  const Line line = make_line(p, span[0]);
-  const long long t0 = span[1] + static_cast<long long>(head * p.row_blocks + rb) * n_tiles;
-  const int c0 = line.owner(t0), c1 = line.owner(t0 + n_tiles - 1);
   if (c0 == c1) return;
-  // the first CTA's share ends inside the unit (its second partial result) unless the unit starts the share; all
-  // later CTAs begin inside the unit
+  // the first CTA's share ends inside the unit (its second partial result); all later CTAs begin inside the unit
   auto slot_of = [&](int c) { return c == c0 ? 2 * c + 1 : 2 * c; };
-  float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, p.part_ml[slot_of(c) * p.rows_per_block + row].x);
-#pragma unroll
-  for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
-  const float m_ref = m == -INFINITY ? 0.f : m;
+  auto ml_of = [&](int c) { return p.part_ml[slot_of(c) * p.rows_per_block + row]; };
+  float2 ml = c0 + lane <= c1 ? ml_of(c0 + lane) : make_float2(-INFINITY, 0.f);
+  float m = ml.x;
+  for (int c = c0 + 32 + lane; c <= c1; c += 32) m = fmaxf(m, ml_of(c).x);
+  m = warp_max(m);
+  const float ref = m == -INFINITY ? 0.f : m;
+  const int grp = tid / kPer, col = col0 + tid % kPer * 4;
+  const float* base = p.part_o + static_cast<int64_t>(row) * kHeadDim + col;
+  const int64_t pitch = static_cast<int64_t>(p.rows_per_block) * kHeadDim;
   float l = 0.f;
-  for (int c = c0 + lane; c <= c1; c += 32) {
-    const float2 ml = p.part_ml[slot_of(c) * p.rows_per_block + row];
-    l += ml.y * ex2(ml.x - m_ref);
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int cc = c0; cc <= c1; cc += 32) {  // lane: weight of partial result cc + lane
+    if (cc > c0) ml = cc + lane <= c1 ? ml_of(cc + lane) : make_float2(-INFINITY, 0.f);
+    const float w = ex2(ml.x - ref);
+    l += w * ml.y;
+    const int n = min(32, c1 - cc + 1);
+#pragma unroll 4
+    for (int k = grp; k < n; k += kGroups) {
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(base + slot_of(cc + k) * pitch));
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      s.x += wk * v.x, s.y += wk * v.y, s.z += wk * v.z, s.w += wk * v.w;
+    }
   }
 #pragma unroll
   for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
-  const int grp = tid >> 7, col = (tid & 127) * 4;
-  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int c = c0 + grp; c <= c1; c += kJoinGroups) {
-    const int64_t at = static_cast<int64_t>(slot_of(c)) * p.rows_per_block + row;
-    const float w = ex2(p.part_ml[at].x - m_ref);
-    const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * kHeadDim + col);
-    s.x += w * v.x, s.y += w * v.y, s.z += w * v.z, s.w += w * v.w;
-  }
-  *reinterpret_cast<float4*>(&acc[grp][col]) = s;
-  __syncthreads();
-  if (grp == 0) {
+  if constexpr (kGroups > 1) {
+    acc[grp][tid % kPer] = s;
+    __syncthreads();
+    if (grp > 0) return;
 #pragma unroll
-    for (int k = 1; k < kJoinGroups; ++k) {
-      const float4 v = *reinterpret_cast<const float4*>(&acc[k][col]);
+    for (int k = 1; k < kGroups; ++k) {
+      const float4 v = acc[k][tid];
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint2 w;
-    w.x = pack2<kFp16>(s.x * inv, s.y * inv), w.y = pack2<kFp16>(s.z * inv, s.w * inv);
-    *reinterpret_cast<uint2*>(out + col) = w;
-    if (tid == 0) {
-      const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
-      if (p.lse) p.lse[lse_at] = l2 * kLn2;
-      if (p.lse2) p.lse2[lse2_at] = l2;
-    }
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint2 w;
+  w.x = pack2<kFp16>(s.x * inv, s.y * inv), w.y = pack2<kFp16>(s.z * inv, s.w * inv);
+  *reinterpret_cast<uint2*>(out + col) = w;
+  if (tid == 0 && col0 == 0) {
+    const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
+    if (p.lse) p.lse[lse_at] = l2 * kLn2;
+    if (p.lse2) p.lse2[lse2_at] = l2;
   }
 }
 
@@ -711,13 +781,21 @@ size_t paged_workspace_bytes(const splitd_paged_params* p) {
 namespace {
 
 template <typename Kernel>
-int raise_smem(Kernel kern, int bytes, std::atomic<int> (&done)[64]) {
+int raise_smem(Kernel kern, int bytes, bool split_regs, std::atomic<int> (&done)[64]) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire)) return 0;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
     cudaGetLastError();
     return fail(SPLITD_ERR_CUDA, "paged attention: the kernel's shared memory cannot be set");
+  }
+  if (split_regs) {
+    cudaFuncAttributes at;
+    if (cudaFuncGetAttributes(&at, kern) != cudaSuccess ||
+        at.numRegs * pa::kThreads < 32 * pa::kProducers * pa::kProducerRegs + pa::kConsumers * pa::kConsumerRegs) {
+      cudaGetLastError();
+      return fail(SPLITD_ERR_CUDA, "paged attention: built with too few registers for its split");
+    }
   }
   if (dev >= 0 && dev < 64) done[dev].store(1, std::memory_order_release);
   return 0;
@@ -727,7 +805,7 @@ template <bool kFp16, int kNB>
 int launch_main(const PagedAttnParams& p, int grid, cudaStream_t stream) {
   static std::atomic<int> done[64];
   auto kern = pa::splitd_paged_attn_kernel<kFp16, kNB>;
-  if (int e = raise_smem(kern, pa::Layout<kNB>::kBytes, done)) return e;
+  if (int e = raise_smem(kern, pa::Layout<kNB>::kBytes, pa::kSplitRegs<kNB>, done)) return e;
   kern<<<grid, pa::kThreads, pa::Layout<kNB>::kBytes, stream>>>(p);
   return 0;
 }
@@ -778,13 +856,24 @@ int launch_paged_attn(const splitd_paged_params* a, cudaStream_t stream) {
     e = fp16 ? launch_main<true, 1>(p, grid, stream) : launch_main<false, 1>(p, grid, stream);
   else if (nb == 2)
     e = fp16 ? launch_main<true, 2>(p, grid, stream) : launch_main<false, 2>(p, grid, stream);
+  else if (nb == 3)
+    e = fp16 ? launch_main<true, 3>(p, grid, stream) : launch_main<false, 3>(p, grid, stream);
   else
     e = fp16 ? launch_main<true, 4>(p, grid, stream) : launch_main<false, 4>(p, grid, stream);
   if (e) return e;
   cudaError_t ce = cudaGetLastError();
-  if (ce == cudaSuccess)
-    ce = launch_dependent(fp16 ? pa::splitd_paged_join_kernel<true> : pa::splitd_paged_join_kernel<false>,
-                          dim3(p.heads_kv * p.rows, p.batch), dim3(pa::kJoinThreads), 0, stream, p);
+  if (ce == cudaSuccess) {
+    // Few units: many CTAs share one, and sixteen groups of threads read their partial results side by side (1 x 131072
+    // keys, 37 results a row: 7 us with four groups, 4 with sixteen).
+    // The choice, which decides the order of the sums, does not look at the width of the page table.
+    const unsigned rows = p.heads_kv * p.rows;
+    if (static_cast<int64_t>(p.batch) * p.heads_kv * p.row_blocks * 8 <= sm_count())
+      ce = launch_dependent(fp16 ? pa::splitd_paged_join_kernel<true, 16, 128> : pa::splitd_paged_join_kernel<false, 16, 128>,
+                            dim3(rows, p.batch, 4), dim3(512), 0, stream, p);
+    else
+      ce = launch_dependent(fp16 ? pa::splitd_paged_join_kernel<true, 1, 512> : pa::splitd_paged_join_kernel<false, 1, 512>,
+                            dim3(rows, p.batch), dim3(128), 0, stream, p);
+  }
   if (ce == cudaSuccess && p.weights) {
     const int64_t longest = max_keys(a) < p.weights_len ? max_keys(a) : p.weights_len;
     ce = launch_dependent(pa::splitd_paged_weights_kernel,
