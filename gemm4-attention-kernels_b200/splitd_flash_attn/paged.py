@@ -36,16 +36,22 @@ from .interface import (
 )
 from .rotary import (
     _DTYPES,
-    _call,
+    _Plans,
     _check_heads,
     _check_inv_freq,
     _check_positions,
     _check_same,
+    _copied,
+    _launch,
+    _meta,
+    _model,
     _position_strides,
-    _rows,
+    _rows_fit,
     _token_strides,
     _traced,
 )
+
+_SCALE = 1.0 / math.sqrt(SUPPORTED_HEAD_DIM)
 
 __all__ = ["split_flash_attn_paged_func", "split_paged_append_func", "split_paged_evict_func"]
 
@@ -81,10 +87,24 @@ def _check_table(page_table, name, batch, device) -> None:
     _check_same(page_table, name, torch.int32, device)
 
 
-def _check_aligned(k_pages, v_pages) -> None:
-    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
-        if t.data_ptr() % 16:
-            raise ValueError(f"{name} must start at a 16-byte boundary")
+def _page_pointers(k_pages, v_pages):
+    k_at, v_at = k_pages.data_ptr(), v_pages.data_ptr()
+    if k_at % 16 or v_at % 16:
+        raise ValueError(("k_pages" if k_at % 16 else "v_pages") + " must start at a 16-byte boundary")
+    return k_at or _NO_MEMORY, v_at or _NO_MEMORY
+
+
+# Stands for the pointer of a tensor without elements, of which nothing is touched; the C-ABI refuses NULL.
+_NO_MEMORY = 256
+
+
+def _fill_cache(p, k_pages, page_table, device) -> None:
+    """What the parameter structs have in common."""
+    p.status_flag = _status_flag(device).data_ptr()
+    p.batch = page_table.shape[0]
+    p.heads_kv, p.head_dim = k_pages.shape[2], SUPPORTED_HEAD_DIM
+    p.num_pages, p.page_size = k_pages.shape[:2]
+    p.max_pages, p.page_table_stride = page_table.shape[1], page_table.stride(0)
 
 
 def _check_weights(key_weights, batch, device) -> None:
@@ -95,8 +115,8 @@ def _check_weights(key_weights, batch, device) -> None:
         raise ValueError("key_weights must have an innermost stride of 1")
 
 
-def _unit_rows(t: torch.Tensor) -> torch.Tensor:
-    return t if t.stride(-1) == 1 else t.contiguous()
+def _unit_rows(*tensors) -> bool:
+    return all(t.stride(-1) == 1 or t.shape[-1] < 2 for t in tensors)
 
 
 # ---------------------------------------------------------------------------
@@ -116,58 +136,62 @@ def _check_paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights) -
         _check_weights(key_weights, q.shape[0], q.device)
 
 
+class _PagedAttnPlan:
+    def __init__(self, q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, causal, left, right, softcap):
+        _check_paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights)
+        causal, local = _resolve_causal_local_window(causal, left, right)
+        batch, sq, hq, _ = q.shape
+        self.index = q.get_device()
+        self.fits = _rows_fit(q) and _unit_rows(page_table, seqlens_k)
+        self.empty = q.numel() == 0
+        self.counted = key_weights is not None and key_weights.shape[1] > 0
+        self.out_model = _model(q.shape, q.dtype, q.device)
+        self.lse_model = _model((batch, hq, sq), torch.float32, q.device)
+        p = _capi.SplitdPagedParams()
+        _fill_cache(p, k_pages, page_table, q.device)
+        p.seqlen_q, p.heads_q, p.dtype = sq, hq, _DTYPES[q.dtype]
+        p.causal, p.local = int(causal), int(local)
+        p.window_left = -1 if left is None or left < 0 else min(left, 2**31 - 1)
+        p.window_right = -1 if right is None or right < 0 else min(right, 2**31 - 1)
+        p.softmax_scale, p.softcap = softmax_scale, softcap
+        p.q_strides, p.o_strides = _token_strides(q), _token_strides(torch.empty_like(self.out_model))
+        p.k_strides, p.v_strides = k_pages.stride()[:3], v_pages.stride()[:3]
+        if self.counted:
+            p.key_weights, p.key_weights_len, p.key_weights_stride = _NO_MEMORY, key_weights.shape[1], key_weights.stride(0)
+        n = 0 if self.empty else _capi.load_library().splitd_paged_attn_workspace_bytes(ctypes.byref(p))
+        p.workspace_bytes = n
+        self.workspace_model = _model((n,), torch.uint8, q.device)
+        self.params = bytes(p)
+
+
+_paged_attn_plans = _Plans()
+
+
 def _paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, causal, left, right, softcap, want_lse):
-    causal, local = _resolve_causal_local_window(causal, left, right)
-    _check_aligned(k_pages, v_pages)
-    device = q.device
-    batch, sq, hq, _ = q.shape
-    q = _rows(q)
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = torch.empty((batch, hq, sq), dtype=torch.float32, device=device) if want_lse else None
-    if out.numel() == 0:
+    how = softmax_scale, causal, left, right, softcap
+    key = (_meta(q), _meta(k_pages), _meta(v_pages), _meta(page_table), _meta(seqlens_k), _meta(key_weights), how)
+    plan = _paged_attn_plans.get(key)
+    if plan is None:
+        plan = _paged_attn_plans.keep(key, _PagedAttnPlan(q, k_pages, v_pages, page_table, seqlens_k, key_weights, *how))
+    q_at = q.data_ptr()
+    if not plan.fits or q_at % 16:
+        return _paged_attn(
+            _copied(q), k_pages, v_pages, page_table.contiguous(), seqlens_k.contiguous(), key_weights, *how, want_lse
+        )
+    out = torch.empty_like(plan.out_model)
+    lse = torch.empty_like(plan.lse_model) if want_lse else None
+    if plan.empty:
         return out, lse
-    page_table, seqlens_k = _unit_rows(page_table), _unit_rows(seqlens_k)
-    lib = _capi.load_library()
-    counted = key_weights is not None and key_weights.shape[1] > 0
-    params = _capi.SplitdPagedParams(
-        q.data_ptr(),
-        k_pages.data_ptr() or 256,  # a cache without pages has no memory, and none of it is touched
-        v_pages.data_ptr() or 256,
-        out.data_ptr(),
-        lse.data_ptr() if want_lse else None,
-        key_weights.data_ptr() if counted else None,
-        page_table.data_ptr() or 256,
-        seqlens_k.data_ptr(),
-        None,
-        0,
-        _status_flag(device).data_ptr(),
-        batch,
-        sq,
-        hq,
-        k_pages.shape[2],
-        SUPPORTED_HEAD_DIM,
-        k_pages.shape[0],
-        k_pages.shape[1],
-        page_table.shape[1],
-        key_weights.shape[1] if counted else 0,
-        _DTYPES[q.dtype],
-        1 if causal else 0,
-        1 if local else 0,
-        -1 if left is None or left < 0 else min(left, 2**31 - 1),
-        -1 if right is None or right < 0 else min(right, 2**31 - 1),
-        softmax_scale,
-        softcap,
-        page_table.stride(0),
-        key_weights.stride(0) if counted else 0,
-        _token_strides(q),
-        _token_strides(out),
-        k_pages.stride()[:3],
-        v_pages.stride()[:3],
-    )
-    n = lib.splitd_paged_attn_workspace_bytes(ctypes.byref(params))
-    workspace = torch.empty(n, dtype=torch.uint8, device=device)
-    params.workspace, params.workspace_bytes = workspace.data_ptr(), n
-    _call(lib.splitd_paged_attn, params, device)
+    workspace = torch.empty_like(plan.workspace_model)
+    p = _capi.SplitdPagedParams.from_buffer_copy(plan.params)
+    p.q, p.o, p.workspace = q_at, out.data_ptr(), workspace.data_ptr()
+    p.k_pages, p.v_pages = _page_pointers(k_pages, v_pages)
+    p.page_table, p.seqlens_k = page_table.data_ptr() or _NO_MEMORY, seqlens_k.data_ptr()
+    if want_lse:
+        p.lse = lse.data_ptr()
+    if plan.counted:
+        p.key_weights = key_weights.data_ptr()
+    _launch(_capi.load_library().splitd_paged_attn, p, plan.index)
     return out, lse
 
 
@@ -185,7 +209,6 @@ def _paged_attn_custom(
     window_size_right: int,
     softcap: float,
 ) -> tuple[torch.Tensor, torch.Tensor]:
-    _check_paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights)
     return _paged_attn(
         q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, causal, _dec(window_size_left),
         _dec(window_size_right), softcap, True,
@@ -231,20 +254,19 @@ def split_flash_attn_paged_func(
     """
     if not isinstance(window_size, tuple) or len(window_size) != 2:
         raise TypeError("window_size must be a tuple of (left, right)")
-    _check_paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights)
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise NotImplementedError("SplitD paged attention has no backward: call it under torch.no_grad() or detach its inputs")
-    softmax_scale = 1.0 / math.sqrt(SUPPORTED_HEAD_DIM) if softmax_scale is None else float(softmax_scale)
-    left, right = window_size
-    if _traced(q, k_pages, v_pages, page_table, seqlens_k, key_weights):
+    softmax_scale = _SCALE if softmax_scale is None else float(softmax_scale)
+    left, right = (None if w is None else int(w) for w in window_size)
+    causal, softcap = bool(causal), float(softcap)
+    if _traced(q, k_pages):
+        _check_paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights)
         out, lse = torch.ops.splitd_flash_attn.paged_attn(
-            q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, bool(causal), _enc(left), _enc(right),
-            float(softcap),
+            q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, causal, _enc(left), _enc(right), softcap
         )
     else:
         out, lse = _paged_attn(
-            q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, bool(causal), left, right,
-            float(softcap), return_lse,
+            q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, causal, left, right, softcap, return_lse
         )
     return (out, lse) if return_lse else out
 
@@ -288,59 +310,70 @@ def _check_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, po
         _check_positions(positions, k.shape[:-2], k.device)
 
 
+class _AppendPlan:
+    def __init__(self, q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q, interleaved, factor):
+        _check_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q)
+        packed = cu_seqlens_q is not None
+        self.index = k.get_device()
+        self.pairs = 0 if inv_freq is None else inv_freq.numel()
+        self.fits = (
+            _rows_fit(q) and _rows_fit(k) and _rows_fit(v) and _unit_rows(page_table, seqlens_k)
+            and (self.pairs < 2 or inv_freq.stride(0) == 1)
+        )
+        self.empty = k.numel() == 0
+        self.q_model = None if q is None else _model(q.shape, q.dtype, q.device)
+        p = _capi.SplitdAppendParams()
+        _fill_cache(p, k_pages, page_table, k.device)
+        p.seqlen, p.total_tokens = (0, k.shape[0]) if packed else (k.shape[1], 0)
+        p.dtype, p.rotary_dim, p.interleaved, p.factor = _DTYPES[k.dtype], 2 * self.pairs, int(interleaved), factor
+        if positions is not None:
+            p.positions_64bit, p.position_strides = int(positions.dtype == torch.int64), _position_strides(positions, packed)
+        if q is not None:
+            p.heads_q, p.q_strides, p.q_out_strides = q.shape[-2], _token_strides(q), _token_strides(torch.empty_like(self.q_model))
+        p.k_strides, p.v_strides = _token_strides(k), _token_strides(v)
+        p.k_page_strides, p.v_page_strides = k_pages.stride()[:3], v_pages.stride()[:3]
+        self.params = bytes(p)
+
+
+_append_plans = _Plans()
+
+
 def _paged_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q, interleaved, factor):
-    _check_aligned(k_pages, v_pages)
-    packed = cu_seqlens_q is not None
-    batch = seqlens_k.shape[0]
-    if packed:
-        _validate_cu_seqlens(cu_seqlens_q, "cu_seqlens_q", batch, total_tokens=k.shape[0])
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if k.numel() == 0:
-        return q_out
-    page_table, seqlens_k = _unit_rows(page_table), _unit_rows(seqlens_k)
-    none = (0, 0, 0)
-    pairs = 0 if inv_freq is None else inv_freq.numel()
-    if pairs:
-        inv_freq = inv_freq.contiguous()
-    lib = _capi.load_library()
-    params = _capi.SplitdAppendParams(
-        q.data_ptr() if q is not None else None,
-        k.data_ptr(),
-        v.data_ptr(),
-        q_out.data_ptr() if q is not None else None,
-        k_pages.data_ptr() or 256,  # see _paged_attn
-        v_pages.data_ptr() or 256,
-        page_table.data_ptr() or 256,
-        seqlens_k.data_ptr() or 256,
-        cu_seqlens_q.data_ptr() if packed else None,
-        positions.data_ptr() if positions is not None else None,
-        inv_freq.data_ptr() if pairs else None,
-        _status_flag(k.device).data_ptr(),
-        batch,
-        0 if packed else k.shape[1],
-        k.shape[0] if packed else 0,
-        q.shape[-2] if q is not None else 0,
-        k.shape[-2],
-        SUPPORTED_HEAD_DIM,
-        k_pages.shape[0],
-        k_pages.shape[1],
-        page_table.shape[1],
-        2 * pairs,
-        1 if interleaved else 0,
-        1 if positions is not None and positions.dtype == torch.int64 else 0,
-        _DTYPES[k.dtype],
-        factor,
-        page_table.stride(0),
-        _position_strides(positions, packed) if positions is not None else (0, 0),
-        _token_strides(q) if q is not None else none,
-        _token_strides(k),
-        _token_strides(v),
-        _token_strides(q_out) if q is not None else none,
-        k_pages.stride()[:3],
-        v_pages.stride()[:3],
+    key = (
+        _meta(q), _meta(k), _meta(v), _meta(k_pages), _meta(v_pages), _meta(page_table), _meta(seqlens_k), _meta(inv_freq),
+        _meta(positions), _meta(cu_seqlens_q), interleaved, factor,
     )
-    _call(lib.splitd_paged_append, params, k.device)
+    plan = _append_plans.get(key)
+    if plan is None:
+        plan = _append_plans.keep(
+            key,
+            _AppendPlan(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q, interleaved, factor),
+        )
+    q_at, k_at, v_at = 0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr()
+    if not plan.fits or q_at % 16 or k_at % 16 or v_at % 16:
+        return _paged_append(
+            None if q is None else _copied(q), _copied(k), _copied(v), k_pages, v_pages, page_table.contiguous(),
+            seqlens_k.contiguous(), None if inv_freq is None else inv_freq.contiguous(), positions, cu_seqlens_q, interleaved,
+            factor,
+        )
+    if cu_seqlens_q is not None:
+        _validate_cu_seqlens(cu_seqlens_q, "cu_seqlens_q", seqlens_k.shape[0], total_tokens=k.shape[0])
+    q_out = None if q is None else torch.empty_like(plan.q_model)
+    if plan.empty:
+        return q_out
+    p = _capi.SplitdAppendParams.from_buffer_copy(plan.params)
+    p.k, p.v = k_at, v_at
+    p.k_pages, p.v_pages = _page_pointers(k_pages, v_pages)
+    p.page_table, p.seqlens_k = page_table.data_ptr() or _NO_MEMORY, seqlens_k.data_ptr() or _NO_MEMORY
+    if q is not None:
+        p.q, p.q_out = q_at, q_out.data_ptr()
+    if plan.pairs:
+        p.inv_freq = inv_freq.data_ptr()
+        if positions is not None:
+            p.positions = positions.data_ptr()
+    if cu_seqlens_q is not None:
+        p.cu_seqlens = cu_seqlens_q.data_ptr()
+    _launch(_capi.load_library().splitd_paged_append, p, plan.index)
     return q_out
 
 
@@ -360,7 +393,6 @@ def _paged_append_custom(
     factor: float,
 ) -> torch.Tensor:
     """The rotated q; an empty tensor if there is none."""
-    _check_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q)
     out = _paged_append(
         q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q, interleaved, factor
     )
@@ -402,15 +434,19 @@ def split_paged_append_func(
     Positions are the slots, unless ``positions`` (one per token, int32 or int64) says otherwise, as it has to after an
     eviction.
     """
-    _check_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, k_pages, v_pages)):
+    if torch.is_grad_enabled() and (
+        k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (q is not None and q.requires_grad)
+    ):
         raise NotImplementedError("SplitD paged append has no backward: call it under torch.no_grad() or detach its inputs")
     interleaved, factor = bool(interleaved), float(factor)
-    args = (q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q)
-    if _traced(*args):
+    if _traced(k, k_pages):
+        args = (q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q)
+        _check_append(*args)
         out = torch.ops.splitd_flash_attn.paged_append(*args, interleaved, factor)
         return None if q is None else out
-    return _paged_append(*args, interleaved, factor)
+    return _paged_append(
+        q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q, interleaved, factor
+    )
 
 
 # ---------------------------------------------------------------------------
@@ -438,46 +474,51 @@ def _check_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_
         )
 
 
+class _EvictPlan:
+    def __init__(self, k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent):
+        _check_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
+        device, batch = k_pages.device, seqlens_k.shape[0]
+        self.index = k_pages.get_device()
+        self.fits = _unit_rows(page_table, new_page_table, seqlens_k)
+        self.empty = batch == 0
+        self.seqlens_model = _model((batch,), torch.int32, device)
+        self.kept_model = _model((batch, keep), torch.int32, device)
+        self.weights_model = _model((batch, keep), torch.float32, device)
+        p = _capi.SplitdEvictParams()
+        _fill_cache(p, k_pages, page_table, device)
+        p.new_max_pages, p.new_page_table_stride = new_page_table.shape[1], new_page_table.stride(0)
+        p.key_weights_len, p.key_weights_stride = key_weights.shape[1], key_weights.stride(0)
+        p.keep, p.keep_first, p.keep_recent = keep, keep_first, keep_recent
+        p.k_strides, p.v_strides = k_pages.stride()[:3], v_pages.stride()[:3]
+        self.params = bytes(p)
+
+
+_evict_plans = _Plans()
+
+
 def _paged_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent):
-    _check_aligned(k_pages, v_pages)
-    device = k_pages.device
-    batch = seqlens_k.shape[0]
-    new_seqlens = torch.empty(batch, dtype=torch.int32, device=device)
-    kept = torch.empty((batch, keep), dtype=torch.int32, device=device)
-    new_weights = torch.empty((batch, keep), dtype=torch.float32, device=device)
-    if batch == 0:
-        return new_seqlens, kept, new_weights
-    page_table, new_page_table, seqlens_k = _unit_rows(page_table), _unit_rows(new_page_table), _unit_rows(seqlens_k)
-    lib = _capi.load_library()
-    params = _capi.SplitdEvictParams(
-        k_pages.data_ptr() or 256,  # see _paged_attn
-        v_pages.data_ptr() or 256,
-        page_table.data_ptr() or 256,
-        new_page_table.data_ptr(),
-        seqlens_k.data_ptr(),
-        key_weights.data_ptr() or 256,
-        new_seqlens.data_ptr(),
-        kept.data_ptr(),
-        new_weights.data_ptr(),
-        _status_flag(device).data_ptr(),
-        batch,
-        k_pages.shape[2],
-        SUPPORTED_HEAD_DIM,
-        k_pages.shape[0],
-        k_pages.shape[1],
-        page_table.shape[1],
-        new_page_table.shape[1],
-        key_weights.shape[1],
-        keep,
-        keep_first,
-        keep_recent,
-        page_table.stride(0),
-        new_page_table.stride(0),
-        key_weights.stride(0),
-        k_pages.stride()[:3],
-        v_pages.stride()[:3],
+    how = keep, keep_first, keep_recent
+    key = (
+        _meta(k_pages), _meta(v_pages), _meta(page_table), _meta(seqlens_k), _meta(key_weights), _meta(new_page_table), how,
+        type(keep), type(keep_first), type(keep_recent),
     )
-    _call(lib.splitd_paged_evict, params, device)
+    plan = _evict_plans.get(key)
+    if plan is None:
+        plan = _evict_plans.keep(key, _EvictPlan(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, *how))
+    if not plan.fits:
+        return _paged_evict(
+            k_pages, v_pages, page_table.contiguous(), seqlens_k.contiguous(), key_weights, new_page_table.contiguous(), *how
+        )
+    new_seqlens = torch.empty_like(plan.seqlens_model)
+    kept, new_weights = torch.empty_like(plan.kept_model), torch.empty_like(plan.weights_model)
+    if plan.empty:
+        return new_seqlens, kept, new_weights
+    p = _capi.SplitdEvictParams.from_buffer_copy(plan.params)
+    p.k_pages, p.v_pages = _page_pointers(k_pages, v_pages)
+    p.page_table, p.new_page_table = page_table.data_ptr() or _NO_MEMORY, new_page_table.data_ptr()
+    p.seqlens_k, p.key_weights = seqlens_k.data_ptr(), key_weights.data_ptr() or _NO_MEMORY
+    p.new_seqlens, p.kept, p.new_weights = new_seqlens.data_ptr(), kept.data_ptr(), new_weights.data_ptr()
+    _launch(_capi.load_library().splitd_paged_evict, p, plan.index)
     return new_seqlens, kept, new_weights
 
 
@@ -493,9 +534,7 @@ def _paged_evict_custom(
     keep_first: int,
     keep_recent: int,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    args = (k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
-    _check_evict(*args)
-    return _paged_evict(*args)
+    return _paged_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
 
 
 @torch.library.register_fake("splitd_flash_attn::paged_evict")
@@ -528,7 +567,7 @@ def split_paged_evict_func(
     ``split_paged_append_func``.
     """
     args = (k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
-    _check_evict(*args)
-    if _traced(*args[:6]):
+    if _traced(k_pages):
+        _check_evict(*args)
         return torch.ops.splitd_flash_attn.paged_evict(*args)
     return _paged_evict(*args)

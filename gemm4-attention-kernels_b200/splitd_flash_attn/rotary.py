@@ -10,7 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _capi
-from .interface import SUPPORTED_HEAD_DIM, _needs_copy
+from .interface import SUPPORTED_HEAD_DIM
 
 __all__ = ["split_rotary_frequencies", "split_rotary_func"]
 
@@ -118,26 +118,56 @@ def _token_strides(t: torch.Tensor):
     return s[:3] if t.ndim == 4 else (0, s[0], s[1])
 
 
-def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """Head rows are moved in 16-byte pieces: unit stride, the others multiples of 8 elements; else a copy."""
-    if t is None:
-        return None
-    t = t.detach()
-    return t.contiguous() if _needs_copy(t) else t
-
-
 def _traced(*tensors) -> bool:
     """Whether the call goes through its custom op: under torch.compile, and for tensors without memory."""
     return torch.compiler.is_compiling() or any(t is not None and type(t) is not torch.Tensor for t in tensors)
 
 
-def _call(fn, params, device) -> None:
-    index = device.index
+# ---------------------------------------------------------------------------
+# plans
+# ---------------------------------------------------------------------------
+# A decode step's kernels take a few microseconds, less than checking a dozen tensors, filling a parameter struct and
+# allocating in Python do. So what a call's shapes, strides, types and options decide is worked out once and kept under
+# exactly those: that the arguments are fine, the filled struct (as bytes; each call puts its pointers into a copy) and
+# models of the outputs. No pointer to and no value of a caller's tensor is part of it.
+
+_PLANS_MOST = 1024
+
+
+class _Plans(dict):
+    def keep(self, key, plan):
+        if len(self) >= _PLANS_MOST:
+            self.clear()
+        self[key] = plan
+        return plan
+
+
+def _meta(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+def _model(shape, dtype, device) -> torch.Tensor:
+    """``empty_like`` of it is a contiguous tensor of that shape and costs half of ``empty``; it has one element itself."""
+    return torch.empty((), dtype=dtype, device=device).expand(shape)
+
+
+def _rows_fit(t: Optional[torch.Tensor]) -> bool:
+    """Head rows are moved in 16-byte pieces: unit stride, the others multiples of 8 elements; other tensors are copied."""
+    return t is None or (t.stride(-1) == 1 and all(s % 8 == 0 for s in t.stride()[:-1]))
+
+
+def _copied(t: torch.Tensor) -> torch.Tensor:
+    return t.detach().clone(memory_format=torch.contiguous_format)
+
+
+def _launch(fn, params, index: int) -> None:
+    """On the current stream of device `index`, whichever device is current."""
+    stream = torch._C._cuda_getCurrentRawStream(index)  # current_stream(index).cuda_stream without the object
     if index == torch.cuda.current_device():
-        code = fn(ctypes.byref(params), torch.cuda.current_stream(index).cuda_stream)
+        code = fn(ctypes.byref(params), stream)
     else:
         with torch.cuda.device(index):
-            code = fn(ctypes.byref(params), torch.cuda.current_stream(index).cuda_stream)
+            code = fn(ctypes.byref(params), stream)
     if code:
         _capi.check(code)
 
@@ -163,48 +193,62 @@ def _check_rotary(q, k, positions, inv_freq) -> None:
     _check_positions(positions, first.shape[:-2], first.device)
 
 
+class _RotaryPlan:
+    def __init__(self, q, k, positions, inv_freq, interleaved, factor, backward):
+        _check_rotary(q, k, positions, inv_freq)
+        first = q if q is not None else k
+        self.index = first.get_device()
+        self.fits = _rows_fit(q) and _rows_fit(k) and (inv_freq.numel() < 2 or inv_freq.stride(0) == 1)
+        self.q_model = None if q is None else _model(q.shape, q.dtype, q.device)
+        self.k_model = None if k is None else _model(k.shape, k.dtype, k.device)
+        packed = first.ndim == 3
+        batch, seqlen = (1, first.shape[0]) if packed else first.shape[:2]
+        heads = [0 if t is None else t.shape[-2] for t in (q, k)]
+        self.has_q, self.has_k = (batch * seqlen * h > 0 for h in heads)
+        self.has_freq = inv_freq.numel() > 0
+        p = _capi.SplitdRotaryParams()
+        p.batch, p.seqlen, p.head_dim = batch, seqlen, SUPPORTED_HEAD_DIM
+        p.heads_q, p.heads_kv = heads
+        p.rotary_dim, p.interleaved, p.backward = 2 * inv_freq.numel(), int(interleaved), int(backward)
+        p.positions_64bit, p.dtype, p.factor = int(positions.dtype == torch.int64), _DTYPES[first.dtype], factor
+        p.position_strides = _position_strides(positions, packed)
+        if q is not None:
+            p.q_strides, p.q_out_strides = _token_strides(q), _token_strides(torch.empty_like(self.q_model))
+        if k is not None:
+            p.k_strides, p.k_out_strides = _token_strides(k), _token_strides(torch.empty_like(self.k_model))
+        self.params = bytes(p)
+
+
+_rotary_plans = _Plans()
+
+
 def _rotary(q, k, positions, inv_freq, interleaved, factor, backward):
     """One launch for both; None stays None."""
-    first = q if q is not None else k
-    q, k = _rows(q), _rows(k)
-    q_out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    packed = first.ndim == 3
-    batch, seqlen = (1, first.shape[0]) if packed else first.shape[:2]
-    heads = ((q.shape[-2] if q is not None else 0), (k.shape[-2] if k is not None else 0))
-    if batch * seqlen * sum(heads) == 0:
-        return q_out, k_out
-    if heads[0] == 0 and q is not None:
-        q = None
-    if heads[1] == 0 and k is not None:
-        k = None
-    inv_freq = inv_freq.contiguous()
-    none = (0, 0, 0)
-    lib = _capi.load_library()
-    params = _capi.SplitdRotaryParams(
-        q.data_ptr() if q is not None else None,
-        k.data_ptr() if k is not None else None,
-        q_out.data_ptr() if q is not None else None,
-        k_out.data_ptr() if k is not None else None,
-        positions.data_ptr(),
-        inv_freq.data_ptr() if inv_freq.numel() else None,
-        batch,
-        seqlen,
-        *heads,
-        SUPPORTED_HEAD_DIM,
-        2 * inv_freq.numel(),
-        1 if interleaved else 0,
-        1 if backward else 0,
-        1 if positions.dtype == torch.int64 else 0,
-        _DTYPES[first.dtype],
-        factor,
-        _position_strides(positions, packed),
-        _token_strides(q) if q is not None else none,
-        _token_strides(k) if k is not None else none,
-        _token_strides(q_out) if q is not None else none,
-        _token_strides(k_out) if k is not None else none,
-    )
-    _call(lib.splitd_rotary, params, first.device)
+    key = (_meta(q), _meta(k), _meta(positions), _meta(inv_freq), interleaved, factor, backward)
+    plan = _rotary_plans.get(key)
+    if plan is None:
+        plan = _rotary_plans.keep(key, _RotaryPlan(q, k, positions, inv_freq, interleaved, factor, backward))
+    q_at = q.data_ptr() if plan.has_q else 0
+    k_at = k.data_ptr() if plan.has_k else 0
+    if not plan.fits or q_at % 16 or k_at % 16:
+        q = None if q is None else _copied(q)
+        k = None if k is None else _copied(k)
+        return _rotary(q, k, positions, inv_freq.contiguous(), interleaved, factor, backward)
+    p = _capi.SplitdRotaryParams.from_buffer_copy(plan.params)
+    q_out = k_out = None
+    if q is not None:
+        q_out = torch.empty_like(plan.q_model)
+    if k is not None:
+        k_out = torch.empty_like(plan.k_model)
+    if plan.has_q:
+        p.q, p.q_out = q_at, q_out.data_ptr()
+    if plan.has_k:
+        p.k, p.k_out = k_at, k_out.data_ptr()
+    if plan.has_q or plan.has_k:
+        p.positions = positions.data_ptr()
+        if plan.has_freq:
+            p.inv_freq = inv_freq.data_ptr()
+        _launch(_capi.load_library().splitd_rotary, p, plan.index)
     return q_out, k_out
 
 
@@ -244,7 +288,6 @@ def _rotary_custom(
     backward: bool,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """An output for an input that is None is an empty tensor."""
-    _check_rotary(q, k, positions, inv_freq)
     q_out, k_out = _rotary(q, k, positions, inv_freq, interleaved, factor, backward)
     none = inv_freq.new_empty((0,), dtype=(q if q is not None else k).dtype)
     return (none if q_out is None else q_out), (none.clone() if k_out is None else k_out)
@@ -293,9 +336,9 @@ def split_rotary_func(
     far positions lose nothing. A pair is dimensions (i, i + rotary_dim / 2), with ``interleaved`` (2 i, 2 i + 1).
     ``factor`` scales what is rotated; the dimensions behind pass through unchanged.
     """
-    _check_rotary(q, k, positions, inv_freq)
     interleaved, factor = bool(interleaved), float(factor)
-    if _traced(q, k, positions, inv_freq):
+    if _traced(q, k):
+        _check_rotary(q, k, positions, inv_freq)
         q_out, k_out = torch.ops.splitd_flash_attn.rotary(q, k, positions, inv_freq, interleaved, factor, False)
         return (None if q is None else q_out), (None if k is None else k_out)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
