@@ -4,11 +4,14 @@
 // Selection. A sequence of n slots keeps m = min(n, keep): its first keep_first and last keep_recent slots, and of the
 // others the m - (those) with the largest weight; of equal weights the lower slot stays. Weights are mapped to 32-bit
 // keys whose order as whole numbers is the order of the weights (-0 = +0, NaN above everything), and the smallest kept
-// key is found digit by digit from the top (8 bits a pass): a histogram of the digit among the keys that agree with the
-// digits found so far, and a scan from its upper end. No sums of weights are formed, so the result is exact.
+// key, the threshold, is found digit by digit from the top (11, 11 and 10 bits): a histogram of the digit among the keys
+// that agree with the digits found so far, and a scan from its upper end. No sums of weights are formed, so the result
+// is exact. A slot's place is then the number of slots above the threshold before it, plus the number of equal ones
+// before it as far as those stay: counts per warp, one scan over warps and CTAs, and a last pass.
 //
-// One cluster of eight CTAs per sequence, each with an eighth of its slots; histograms and counts meet through
-// distributed shared memory. A last pass over the slots gives every kept one its place by a running count.
+// A cluster of eight CTAs per sequence, each with an eighth of its slots; histograms and counts meet through distributed
+// shared memory. Up to kOneCta slots a single CTA is faster than the cluster's barriers. The weights are read once and
+// their keys kept in shared memory (a sequence of more than eight times kCacheMost slots is read from L2 again). What bounds it is the chain of passes and barriers (131072 slots: ... us), not bytes.
 //
 // Copy. One warp per kept slot and tensor, 16 bytes per lane, four head rows in flight; nothing is read or written
 // that does not move. It is bound by HBM: 2 * heads_kv KB read and written per slot.
@@ -24,8 +27,11 @@ namespace sd {
 
 namespace ev {
 constexpr int kCluster = 8;
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kOneCta = 8192;
+constexpr int kCacheMost = 49152;  // keys that a CTA keeps in shared memory (192 KB)
 constexpr int kCopyWarps = 8;
 constexpr int kCopyUnroll = 4;
 }  // namespace ev
@@ -45,6 +51,7 @@ struct EvictParams {
   int* kept;          // (batch, keep), -1 behind the last one
   float* new_weights; // (batch, keep), 0 behind the last one
   int* status;
+  int cached;  // keys a CTA has room for in shared memory
 };
 
 namespace ev {
@@ -59,147 +66,152 @@ __device__ __forceinline__ int cache_len(const EvictParams& p, int b) {
   return min(min(max(__ldg(p.seqlens + b), 0), page_capacity(p.from)), p.weights_len);
 }
 
-__device__ __forceinline__ int block_sum(int v, int* scratch, int warp, int lane) {
-  v = __reduce_add_sync(0xffffffffu, v);
-  __syncthreads();
-  if (lane == 0) scratch[warp] = v;
-  __syncthreads();
-  int s = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) s += scratch[i];
-  return s;
-}
-
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kThreads) splitd_evict_select_kernel(const __grid_constant__ EvictParams p) {
+template <int kCtas>
+__global__ void __launch_bounds__(kThreads) splitd_evict_select_kernel(const __grid_constant__ EvictParams p) {
+  extern __shared__ uint32_t cache[];  // keys of this CTA's slots
   namespace cg = cooperative_groups;
-  __shared__ unsigned hist[256];
-  __shared__ unsigned total[256];
-  __shared__ int scratch[kWarps];
-  __shared__ int counts[2];  // kept for certain, equal to the threshold: of this CTA's slots
+  __shared__ unsigned hist[kBins];   // of this CTA
+  __shared__ unsigned total[kBins];  // of the cluster
+  __shared__ unsigned warp_total[kWarps];
   __shared__ unsigned found[2];
+  __shared__ int counts[2];  // this CTA's slots above the threshold and equal to it
+  __shared__ int2 warp_counts[kWarps];
   cg::cluster_group cluster = cg::this_cluster();
+  auto cluster_sync = [&] {
+    if constexpr (kCtas > 1) cluster.sync(); else __syncthreads();
+  };
   pdl_launch_dependents();
-  const int b = blockIdx.x / kCluster, rank = cluster.block_rank();
+  const int b = blockIdx.x / kCtas, rank = kCtas > 1 ? static_cast<int>(cluster.block_rank()) : 0;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int n = cache_len(p, b);
   if (rank == 0 && tid == 0 && p.status && __ldg(p.seqlens + b) > n) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
   const int m = min(n, p.keep);
+  const bool all = n <= p.keep;
   const float* w = p.weights + b * p.weights_stride;
   // slots in [lo, hi) compete for the places that the first and the recent ones leave
   const int lo = min(p.keep_first, n), hi = max(lo, n - p.keep_recent);
-  const int per = ((hi - lo) + kCluster - 1) / kCluster;
+  const int per = ((hi - lo) + kCtas - 1) / kCtas;
   const int c0 = min(lo + rank * per, hi), c1 = min(c0 + per, hi);
-  int want = m - (n - (hi - lo));  // of [lo, hi)
+  const bool cached = c1 - c0 <= p.cached;
+  auto key_at = [&](int i) { return cached ? cache[i - c0] : order_key(__ldg(w + i)); };
+  int want = m - (n - (hi - lo));  // of [lo, hi); at the end: of those equal to the threshold
   uint32_t threshold = 0;
-  if (n <= p.keep) {
-    want = hi - lo;  // everything stays (threshold 0: no key is below it)
-  } else {
+  int above = 0;  // of this CTA, spread over its threads
+  if (!all) {
     uint32_t mask = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kThreads) hist[i] = 0;
+    const int shifts[3] = {21, 10, 0};
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = shifts[pass];
+      const uint32_t digit_mask = pass < 2 ? 2047u : 1023u;
+      hist[tid] = 0, hist[tid + kThreads] = 0;
       __syncthreads();
-      for (int i0 = c0; i0 < c1; i0 += kThreads) {
-        const int i = i0 + tid;
-        const uint32_t key = i < c1 ? order_key(__ldg(w + i)) : 0u;
-        const bool in = i < c1 && (key & mask) == threshold;
-        const unsigned active = __ballot_sync(0xffffffffu, in);
-        if (in) {
-          const uint32_t digit = (key >> shift) & 255u;
-          const unsigned same = __match_any_sync(active, digit);
-          if (lane == __ffs(same) - 1) atomicAdd(hist + digit, __popc(same));
+#pragma unroll 8
+      for (int i = c0 + tid; i < c1; i += kThreads) {
+        uint32_t key;
+        if (pass == 0) {
+          key = order_key(__ldg(w + i));
+          if (cached) cache[i - c0] = key;
+        } else {
+          key = key_at(i);
         }
+        if ((key & mask) == threshold) atomicAdd(hist + ((key >> shift) & digit_mask), 1u);
       }
-      cluster.sync();
-      if (tid < 256) {
-        unsigned s = 0;
+      cluster_sync();
+      if constexpr (kCtas > 1) {
+        if (tid < kBins / kCtas) {
+          const int bin = rank * (kBins / kCtas) + tid;
+          unsigned s = 0;
 #pragma unroll
-        for (int r = 0; r < kCluster; ++r) s += cluster.map_shared_rank(hist, r)[tid];
-        total[tid] = s;
-      }
-      cluster.sync();  // every CTA has read the histograms
-      // from the top: the digit in which the running count reaches `want`
-      if (warp == 0) {
-        unsigned mine[8], sum = 0;
+          for (int r = 0; r < kCtas; ++r) s += cluster.map_shared_rank(hist, r)[bin];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum += mine[e] = total[255 - (lane * 8 + e)];
-        unsigned incl = sum;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-          const unsigned o = __shfl_up_sync(0xffffffffu, incl, d);
-          if (lane >= d) incl += o;
+          for (int r = 0; r < kCtas; ++r) cluster.map_shared_rank(total, r)[bin] = s;
         }
-        unsigned above = incl - sum;
-        if (above < static_cast<unsigned>(want) && incl >= static_cast<unsigned>(want)) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (above < static_cast<unsigned>(want) && above + mine[e] >= static_cast<unsigned>(want))
-              found[0] = 255 - (lane * 8 + e), found[1] = above;
-            above += mine[e];
-          }
-        }
-        if (want == 0 && lane == 0) found[0] = 255, found[1] = 0;
+        cluster_sync();
       }
+      // from the top: the digit in which the running count reaches `want`; thread t has the t-th pair of bins from there
+      const unsigned* sum = kCtas > 1 ? total : hist;
+      const int top = kBins - 1 - 2 * tid;
+      const unsigned n0 = sum[top], n1 = sum[top - 1];
+      unsigned incl = n0 + n1;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const unsigned o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += o;
+      }
+      if (lane == 31) warp_total[warp] = incl;
+      if (tid == 0) found[0] = digit_mask, found[1] = 0;  // want == 0: above every key
       __syncthreads();
-      threshold |= found[0] << shift;
-      mask |= 255u << shift;
+      unsigned before = lane < warp ? warp_total[lane] : 0u;
+      before = __reduce_add_sync(0xffffffffu, before) + incl - (n0 + n1);
+      const unsigned goal = static_cast<unsigned>(want);
+      if (before < goal && before + n0 >= goal)
+        found[0] = top, found[1] = before;
+      else if (before + n0 < goal && before + n0 + n1 >= goal)
+        found[0] = top - 1, found[1] = before + n0;
+      __syncthreads();
+      const unsigned digit = found[0];
       want -= static_cast<int>(found[1]);
+      threshold |= digit << shift;
+      mask |= digit_mask << shift;
+      above += (top > static_cast<int>(digit) ? hist[top] : 0u) + (top - 1 > static_cast<int>(digit) ? hist[top - 1] : 0u);
+      if (pass == 2 && tid == 0) counts[1] = static_cast<int>(hist[digit]);
       __syncthreads();
     }
   }
-  // `want` slots of weight `threshold` stay, and every slot above it
-  const bool all = n <= p.keep;
-  int above = 0, equal = 0;
-  for (int i = c0 + tid; i < c1; i += kThreads) {
-    const uint32_t key = order_key(__ldg(w + i));
-    above += all || key > threshold, equal += !all && key == threshold;
+  // counts of this CTA, of the CTAs before it, and of the warps before this one; a warp has a run of neighbouring slots
+  above = __reduce_add_sync(0xffffffffu, above);
+  if (lane == 0) warp_total[warp] = above;
+  __syncthreads();
+  if (warp == 0) {
+    const int s = __reduce_add_sync(0xffffffffu, static_cast<int>(warp_total[lane]));
+    if (lane == 0) {
+      counts[0] = all ? c1 - c0 : s;
+      if (all) counts[1] = 0;
+    }
   }
-  above = block_sum(above, scratch, warp, lane);
-  equal = block_sum(equal, scratch, warp, lane);
-  if (tid == 0) counts[0] = above, counts[1] = equal;
-  cluster.sync();
-  int place = lo, eq = 0;  // place of this CTA's first kept slot; slots equal to the threshold before this CTA's
-  for (int r = 0; r < rank; ++r) {
-    const int* c = cluster.map_shared_rank(counts, r);
-    place += c[0] + min(max(want - eq, 0), c[1]), eq += c[1];
+  const int run = ((c1 - c0 + kWarps - 1) / kWarps + 31) / 32 * 32;
+  const int w0 = min(c0 + warp * run, c1), w1 = min(w0 + run, c1);
+  int a_mine = 0, e_mine = 0;
+#pragma unroll 4
+  for (int i = w0 + lane; i < w1; i += 32) {
+    const uint32_t key = all ? 0u : key_at(i);
+    a_mine += all || key > threshold, e_mine += !all && key == threshold;
   }
-  cluster.sync();  // nobody reads the counts of a CTA that has ended
+  a_mine = __reduce_add_sync(0xffffffffu, a_mine), e_mine = __reduce_add_sync(0xffffffffu, e_mine);
+  if (lane == 0) warp_counts[warp] = make_int2(a_mine, e_mine);
+  cluster_sync();
+  int a = 0, e = 0;
+  {
+    const int2 c = lane < warp ? warp_counts[lane] : make_int2(0, 0);
+    a = c.x, e = c.y;
+    if constexpr (kCtas > 1) {
+      if (lane < rank) {
+        const int* other = cluster.map_shared_rank(counts, lane);
+        a += other[0], e += other[1];
+      }
+    }
+    a = __reduce_add_sync(0xffffffffu, a), e = __reduce_add_sync(0xffffffffu, e);
+  }
+  cluster_sync();  // nobody reads the counts of a CTA that has ended
   int* kept = p.kept + static_cast<int64_t>(b) * p.keep;
   float* nw = p.new_weights + static_cast<int64_t>(b) * p.keep;
-  for (int i0 = c0; i0 < c1; i0 += kThreads) {
-    const int i = i0 + tid;
-    const float v = i < c1 ? __ldg(w + i) : 0.f;
-    const uint32_t key = order_key(v);
-    const bool is_above = i < c1 && (all || key > threshold), is_equal = i < c1 && !all && key == threshold;
-    const unsigned em = __ballot_sync(0xffffffffu, is_equal), below = (1u << lane) - 1;
-    // counts of the warps before this one: equal ones first, since they decide which of them stay
-    __syncthreads();
-    if (lane == 0) scratch[warp] = __popc(em);
-    __syncthreads();
-    int eq_before = eq, eq_all = 0;
-#pragma unroll
-    for (int k = 0; k < kWarps; ++k) {
-      if (k < warp) eq_before += scratch[k];
-      eq_all += scratch[k];
+  const unsigned below = (1u << lane) - 1;
+#pragma unroll 4
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t key = i < w1 && !all ? key_at(i) : 0u;
+    const bool is_above = i < w1 && (all || key > threshold), is_equal = i < w1 && !all && key == threshold;
+    const unsigned am = __ballot_sync(0xffffffffu, is_above), em = __ballot_sync(0xffffffffu, is_equal);
+    const int my_e = e + __popc(em & below);
+    if (is_above || (is_equal && my_e < want)) {
+      const int at = lo + a + __popc(am & below) + min(my_e, want);
+      kept[at] = i, nw[at] = __ldg(w + i);
     }
-    const bool stays = is_above || (is_equal && eq_before + __popc(em & below) < want);
-    const unsigned sm = __ballot_sync(0xffffffffu, stays);
-    __syncthreads();
-    if (lane == 0) scratch[warp] = __popc(sm);
-    __syncthreads();
-    int at = place, st_all = 0;
-#pragma unroll
-    for (int k = 0; k < kWarps; ++k) {
-      if (k < warp) at += scratch[k];
-      st_all += scratch[k];
-    }
-    if (stays) {
-      at += __popc(sm & below);
-      kept[at] = i, nw[at] = v;
-    }
-    place += st_all, eq += eq_all;
+    a += __popc(am), e += __popc(em);
   }
   // the first and the recent ones, and the empty places behind them
-  const int gtid = rank * kThreads + tid, step = kCluster * kThreads;
+  const int gtid = rank * kThreads + tid, step = kCtas * kThreads;
   for (int i = gtid; i < lo; i += step) kept[i] = i, nw[i] = __ldg(w + i);
   for (int i = hi + gtid; i < n; i += step) kept[m - (n - i)] = i, nw[m - (n - i)] = __ldg(w + i);
   for (int i = m + gtid; i < p.keep; i += step) kept[i] = -1, nw[i] = 0.f;
@@ -247,6 +259,25 @@ __global__ void __launch_bounds__(kCopyWarps * 32) splitd_evict_copy_kernel(cons
 
 }  // namespace ev
 
+namespace {
+
+// once per device and kernel
+int allow_cache(void (*kern)(EvictParams), bool one) {
+  static std::atomic<int> done[2][64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const bool known = dev >= 0 && dev < 64;
+  if (known && done[one][dev].load(std::memory_order_acquire)) return 0;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, ev::kCacheMost * 4) != cudaSuccess) {
+    cudaGetLastError();
+    return fail(SPLITD_ERR_CUDA, "eviction: the kernel's shared memory cannot be set");
+  }
+  if (known) done[one][dev].store(1, std::memory_order_release);
+  return 0;
+}
+
+}  // namespace
+
 int launch_evict(const splitd_evict_params* a, cudaStream_t stream) {
   EvictParams p;
   memset(&p, 0, sizeof(p));
@@ -263,8 +294,24 @@ int launch_evict(const splitd_evict_params* a, cudaStream_t stream) {
   p.keep = a->keep, p.keep_first = a->keep_first, p.keep_recent = a->keep_recent;
   p.new_seqlens = a->new_seqlens, p.kept = a->kept, p.new_weights = a->new_weights;
   p.status = a->status_flag;
-  ev::splitd_evict_select_kernel<<<dim3(a->batch * ev::kCluster), ev::kThreads, 0, stream>>>(p);
-  cudaError_t ce = cudaGetLastError();
+  int64_t slots = static_cast<int64_t>(a->max_pages) * a->page_size;
+  if (a->key_weights_len < slots) slots = a->key_weights_len;
+  const bool one = slots <= ev::kOneCta;
+  const int64_t share = one ? slots : (slots + ev::kCluster - 1) / ev::kCluster;
+  p.cached = static_cast<int>(share < ev::kCacheMost ? share : ev::kCacheMost);
+  if (int e = allow_cache(one ? ev::splitd_evict_select_kernel<1> : ev::splitd_evict_select_kernel<ev::kCluster>, one)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(one ? a->batch : a->batch * ev::kCluster);
+  cfg.blockDim = dim3(ev::kThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.cached) * 4;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = ev::kCluster, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = one ? 0 : 1;
+  cudaError_t ce = one ? cudaLaunchKernelEx(&cfg, ev::splitd_evict_select_kernel<1>, p)
+                       : cudaLaunchKernelEx(&cfg, ev::splitd_evict_select_kernel<ev::kCluster>, p);
   if (ce == cudaSuccess)
     ce = launch_dependent(ev::splitd_evict_copy_kernel,
                           dim3((a->keep + ev::kCopyWarps / 2 - 1) / (ev::kCopyWarps / 2), a->batch),

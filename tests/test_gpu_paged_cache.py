@@ -214,6 +214,25 @@ def test_evict_long():
     check_evict(lens, 4001, 16, 300, 1, 64, torch.bfloat16, some_weights(lens, "plain"))
 
 
+@pytest.mark.parametrize("kind", ["plain", "ties"])
+def test_evict_longer_than_the_keys_in_shared_memory(kind):
+    """More than 8 x 49152 slots; page table entries all name the same few pages (reading shared pages is fine)."""
+    from splitd_flash_attn import split_paged_evict_func
+
+    n, keep = 500001, 1003
+    k = torch.randn(10, 1000, 1, D, device="cuda").to(torch.bfloat16)
+    v = torch.randn(10, 1000, 1, D, device="cuda").to(torch.bfloat16)
+    table = (torch.arange(501, device="cuda", dtype=torch.int32) % 8)[None]
+    new = torch.tensor([[8, 9]], device="cuda", dtype=torch.int32)
+    w = some_weights([n], kind, 5)
+    m, kept, nw = split_paged_evict_func(k, v, table, torch.tensor([n], device="cuda", dtype=torch.int32), w, new, keep, 1, 2)
+    s = torch.tensor(evict_ref(w, [n], keep, 1, 2)[0], device="cuda")
+    assert int(m) == keep and torch.equal(kept[0].long(), s) and torch.equal(nw[0], w[0, s])
+    flat = k.view(-1, D)
+    assert torch.equal(flat[8000 : 8000 + keep], flat[s // 1000 % 8 * 1000 + s % 1000])
+    assert_status_ok()
+
+
 def test_evict_bad_pages_and_lengths():
     from splitd_flash_attn import split_paged_evict_func
     from splitd_flash_attn.interface import kernel_status, reset_kernel_status
