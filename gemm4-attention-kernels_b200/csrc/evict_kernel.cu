@@ -9,9 +9,10 @@
 // is exact. A slot's place is then the number of slots above the threshold before it, plus the number of equal ones
 // before it as far as those stay: counts per warp, one scan over warps and CTAs, and a last pass.
 //
-// A cluster of eight CTAs per sequence, each with an eighth of its slots; histograms and counts meet through distributed
+// A cluster of eight CTAs per sequence, each with its share of the slots; histograms and counts meet through distributed
 // shared memory. Up to kOneCta slots a single CTA is faster than the cluster's barriers. The weights are read once and
-// their keys kept in shared memory (a sequence of more than eight times kCacheMost slots is read from L2 again). What bounds it is the chain of passes and barriers (131072 slots: ... us), not bytes.
+// their keys kept in shared memory (a sequence of more than eight times kCacheMost slots is read from L2 again). What bounds it is the chain of passes and barriers (131072 slots: 19 us;
+// the copy of 20000 of them, 4 heads: 50 us), not bytes.
 //
 // Copy. One warp per kept slot and tensor, 16 bytes per lane, four head rows in flight; nothing is read or written
 // that does not move. It is bound by HBM: 2 * heads_kv KB read and written per slot.
@@ -26,7 +27,7 @@
 namespace sd {
 
 namespace ev {
-constexpr int kCluster = 8;
+constexpr int kCluster = 8;  // sixteen: the same time for one sequence of 131072 slots, 14 % more for 8 of 16384
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
@@ -77,145 +78,144 @@ __global__ void __launch_bounds__(kThreads) splitd_evict_select_kernel(const __g
   __shared__ int counts[2];  // this CTA's slots above the threshold and equal to it
   __shared__ int2 warp_counts[kWarps];
   cg::cluster_group cluster = cg::this_cluster();
-  auto cluster_sync = [&] {
-    if constexpr (kCtas > 1) cluster.sync(); else __syncthreads();
-  };
   pdl_launch_dependents();
   const int b = blockIdx.x / kCtas, rank = kCtas > 1 ? static_cast<int>(cluster.block_rank()) : 0;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int gtid = rank * kThreads + tid, step = kCtas * kThreads;
   const int n = cache_len(p, b);
-  if (rank == 0 && tid == 0 && p.status && __ldg(p.seqlens + b) > n) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
   const int m = min(n, p.keep);
-  const bool all = n <= p.keep;
-  const float* w = p.weights + b * p.weights_stride;
+  if (gtid == 0) {
+    p.new_seqlens[b] = m;
+    if (p.status && __ldg(p.seqlens + b) > n) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
+  }
+  int* kept = p.kept + static_cast<int64_t>(b) * p.keep;
+  for (int i = m + gtid; i < p.keep; i += step) kept[i] = -1;
+  if (n <= p.keep) {  // the whole cluster: everything stays
+    for (int i = gtid; i < n; i += step) kept[i] = i;
+    return;
+  }
   // slots in [lo, hi) compete for the places that the first and the recent ones leave
-  const int lo = min(p.keep_first, n), hi = max(lo, n - p.keep_recent);
+  const int lo = p.keep_first, hi = n - p.keep_recent;
+  for (int i = gtid; i < lo; i += step) kept[i] = i;
+  for (int i = hi + gtid; i < n; i += step) kept[m - (n - i)] = i;
+  const float* w = p.weights + b * p.weights_stride;
   const int per = ((hi - lo) + kCtas - 1) / kCtas;
   const int c0 = min(lo + rank * per, hi), c1 = min(c0 + per, hi);
   const bool cached = c1 - c0 <= p.cached;
-  auto key_at = [&](int i) { return cached ? cache[i - c0] : order_key(__ldg(w + i)); };
   int want = m - (n - (hi - lo));  // of [lo, hi); at the end: of those equal to the threshold
-  uint32_t threshold = 0;
+  uint32_t threshold = 0, mask = 0;
   int above = 0;  // of this CTA, spread over its threads
-  if (!all) {
-    uint32_t mask = 0;
-    const int shifts[3] = {21, 10, 0};
+  constexpr int kShift[3] = {21, 10, 0};
 #pragma unroll
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = shifts[pass];
-      const uint32_t digit_mask = pass < 2 ? 2047u : 1023u;
-      hist[tid] = 0, hist[tid + kThreads] = 0;
-      __syncthreads();
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = kShift[pass];
+    const uint32_t digit_mask = pass < 2 ? 2047u : 1023u;
+    hist[tid] = 0, hist[tid + kThreads] = 0;
+    __syncthreads();
+    auto count = [&](uint32_t key) {
+      if ((key & mask) == threshold) atomicAdd(hist + ((key >> shift) & digit_mask), 1u);
+    };
+    if (pass > 0 && cached) {
+#pragma unroll 4
+      for (int i = tid; i < c1 - c0; i += kThreads) count(cache[i]);
+    } else {
 #pragma unroll 8
-      for (int i = c0 + tid; i < c1; i += kThreads) {
-        uint32_t key;
-        if (pass == 0) {
-          key = order_key(__ldg(w + i));
-          if (cached) cache[i - c0] = key;
-        } else {
-          key = key_at(i);
-        }
-        if ((key & mask) == threshold) atomicAdd(hist + ((key >> shift) & digit_mask), 1u);
+      for (int i = tid; i < c1 - c0; i += kThreads) {
+        const uint32_t key = order_key(__ldg(w + c0 + i));
+        if (cached) cache[i] = key;
+        count(key);
       }
-      cluster_sync();
-      if constexpr (kCtas > 1) {
-        if (tid < kBins / kCtas) {
-          const int bin = rank * (kBins / kCtas) + tid;
-          unsigned s = 0;
+    }
+    if constexpr (kCtas > 1) {
+      cluster.sync();
+      if (tid < kBins / kCtas) {
+        const int bin = rank * (kBins / kCtas) + tid;
+        unsigned s = 0;
 #pragma unroll
-          for (int r = 0; r < kCtas; ++r) s += cluster.map_shared_rank(hist, r)[bin];
+        for (int r = 0; r < kCtas; ++r) s += cluster.map_shared_rank(hist, r)[bin];
 #pragma unroll
-          for (int r = 0; r < kCtas; ++r) cluster.map_shared_rank(total, r)[bin] = s;
-        }
-        cluster_sync();
+        for (int r = 0; r < kCtas; ++r) cluster.map_shared_rank(total, r)[bin] = s;
       }
-      // from the top: the digit in which the running count reaches `want`; thread t has the t-th pair of bins from there
-      const unsigned* sum = kCtas > 1 ? total : hist;
-      const int top = kBins - 1 - 2 * tid;
-      const unsigned n0 = sum[top], n1 = sum[top - 1];
-      unsigned incl = n0 + n1;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const unsigned o = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += o;
-      }
-      if (lane == 31) warp_total[warp] = incl;
-      if (tid == 0) found[0] = digit_mask, found[1] = 0;  // want == 0: above every key
-      __syncthreads();
-      unsigned before = lane < warp ? warp_total[lane] : 0u;
-      before = __reduce_add_sync(0xffffffffu, before) + incl - (n0 + n1);
-      const unsigned goal = static_cast<unsigned>(want);
-      if (before < goal && before + n0 >= goal)
-        found[0] = top, found[1] = before;
-      else if (before + n0 < goal && before + n0 + n1 >= goal)
-        found[0] = top - 1, found[1] = before + n0;
-      __syncthreads();
-      const unsigned digit = found[0];
-      want -= static_cast<int>(found[1]);
-      threshold |= digit << shift;
-      mask |= digit_mask << shift;
-      above += (top > static_cast<int>(digit) ? hist[top] : 0u) + (top - 1 > static_cast<int>(digit) ? hist[top - 1] : 0u);
-      if (pass == 2 && tid == 0) counts[1] = static_cast<int>(hist[digit]);
+      cluster.sync();
+    } else {
       __syncthreads();
     }
+    // from the top: the digit in which the running count reaches `want`; thread t has the t-th pair of bins from there
+    const unsigned* sum = kCtas > 1 ? total : hist;
+    const int top = kBins - 1 - 2 * tid;
+    const unsigned n0 = sum[top], n1 = sum[top - 1];
+    unsigned incl = n0 + n1;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const unsigned o = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += o;
+    }
+    if (lane == 31) warp_total[warp] = incl;
+    if (tid == 0) found[0] = digit_mask, found[1] = 0;  // want == 0: above every key
+    __syncthreads();
+    unsigned before = lane < warp ? warp_total[lane] : 0u;
+    before = __reduce_add_sync(0xffffffffu, before) + incl - (n0 + n1);
+    const unsigned goal = static_cast<unsigned>(want);
+    if (before < goal && before + n0 >= goal)
+      found[0] = top, found[1] = before;
+    else if (before + n0 < goal && before + n0 + n1 >= goal)
+      found[0] = top - 1, found[1] = before + n0;
+    __syncthreads();
+    const unsigned digit = found[0];
+    want -= static_cast<int>(found[1]);
+    threshold |= digit << shift;
+    mask |= digit_mask << shift;
+    above += (top > static_cast<int>(digit) ? hist[top] : 0u) + (top - 1 > static_cast<int>(digit) ? hist[top - 1] : 0u);
+    if (pass == 2 && tid == 0) counts[1] = static_cast<int>(hist[digit]);
+    __syncthreads();
   }
   // counts of this CTA, of the CTAs before it, and of the warps before this one; a warp has a run of neighbouring slots
   above = __reduce_add_sync(0xffffffffu, above);
   if (lane == 0) warp_total[warp] = above;
-  __syncthreads();
-  if (warp == 0) {
-    const int s = __reduce_add_sync(0xffffffffu, static_cast<int>(warp_total[lane]));
-    if (lane == 0) {
-      counts[0] = all ? c1 - c0 : s;
-      if (all) counts[1] = 0;
-    }
-  }
   const int run = ((c1 - c0 + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int w0 = min(c0 + warp * run, c1), w1 = min(w0 + run, c1);
-  int a_mine = 0, e_mine = 0;
+  const int w0 = min(warp * run, c1 - c0), w1 = min(w0 + run, c1 - c0);
+  int2 mine = make_int2(0, 0);
+  auto tally = [&](uint32_t key) { mine.x += key > threshold, mine.y += key == threshold; };
+  if (cached) {
 #pragma unroll 4
-  for (int i = w0 + lane; i < w1; i += 32) {
-    const uint32_t key = all ? 0u : key_at(i);
-    a_mine += all || key > threshold, e_mine += !all && key == threshold;
+    for (int i = w0 + lane; i < w1; i += 32) tally(cache[i]);
+  } else {
+#pragma unroll 4
+    for (int i = w0 + lane; i < w1; i += 32) tally(order_key(__ldg(w + c0 + i)));
   }
-  a_mine = __reduce_add_sync(0xffffffffu, a_mine), e_mine = __reduce_add_sync(0xffffffffu, e_mine);
-  if (lane == 0) warp_counts[warp] = make_int2(a_mine, e_mine);
-  cluster_sync();
-  int a = 0, e = 0;
-  {
-    const int2 c = lane < warp ? warp_counts[lane] : make_int2(0, 0);
-    a = c.x, e = c.y;
-    if constexpr (kCtas > 1) {
-      if (lane < rank) {
-        const int* other = cluster.map_shared_rank(counts, lane);
-        a += other[0], e += other[1];
-      }
+  mine.x = __reduce_add_sync(0xffffffffu, mine.x), mine.y = __reduce_add_sync(0xffffffffu, mine.y);
+  if (lane == 0) warp_counts[warp] = mine;
+  __syncthreads();
+  int2 c = lane < warp ? warp_counts[lane] : make_int2(0, 0);
+  if constexpr (kCtas > 1) {
+    if (warp == 0) {
+      const int s = __reduce_add_sync(0xffffffffu, static_cast<int>(warp_total[lane]));
+      if (lane == 0) counts[0] = s;
     }
-    a = __reduce_add_sync(0xffffffffu, a), e = __reduce_add_sync(0xffffffffu, e);
+    cluster.sync();
+    if (lane < rank) {
+      const int* other = cluster.map_shared_rank(counts, lane);
+      c.x += other[0], c.y += other[1];
+    }
   }
-  cluster_sync();  // nobody reads the counts of a CTA that has ended
-  int* kept = p.kept + static_cast<int64_t>(b) * p.keep;
-  float* nw = p.new_weights + static_cast<int64_t>(b) * p.keep;
+  int a = __reduce_add_sync(0xffffffffu, c.x), e = __reduce_add_sync(0xffffffffu, c.y);
+  if constexpr (kCtas > 1) cluster.barrier_arrive();  // done with the others' memory
   const unsigned below = (1u << lane) - 1;
-#pragma unroll 4
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t key = i < w1 && !all ? key_at(i) : 0u;
-    const bool is_above = i < w1 && (all || key > threshold), is_equal = i < w1 && !all && key == threshold;
+  auto place = [&](int i, uint32_t key) {
+    const bool is_above = i < w1 && key > threshold, is_equal = i < w1 && key == threshold;
     const unsigned am = __ballot_sync(0xffffffffu, is_above), em = __ballot_sync(0xffffffffu, is_equal);
     const int my_e = e + __popc(em & below);
-    if (is_above || (is_equal && my_e < want)) {
-      const int at = lo + a + __popc(am & below) + min(my_e, want);
-      kept[at] = i, nw[at] = __ldg(w + i);
-    }
+    if (is_above || (is_equal && my_e < want)) kept[lo + a + __popc(am & below) + min(my_e, want)] = c0 + i;
     a += __popc(am), e += __popc(em);
+  };
+  if (cached) {
+#pragma unroll 4
+    for (int i0 = w0; i0 < w1; i0 += 32) place(i0 + lane, i0 + lane < w1 ? cache[i0 + lane] : 0u);
+  } else {
+#pragma unroll 4
+    for (int i0 = w0; i0 < w1; i0 += 32) place(i0 + lane, i0 + lane < w1 ? order_key(__ldg(w + c0 + i0 + lane)) : 0u);
   }
-  // the first and the recent ones, and the empty places behind them
-  const int gtid = rank * kThreads + tid, step = kCtas * kThreads;
-  for (int i = gtid; i < lo; i += step) kept[i] = i, nw[i] = __ldg(w + i);
-  for (int i = hi + gtid; i < n; i += step) kept[m - (n - i)] = i, nw[m - (n - i)] = __ldg(w + i);
-  for (int i = m + gtid; i < p.keep; i += step) kept[i] = -1, nw[i] = 0.f;
-  if (gtid == 0) p.new_seqlens[b] = m;
+  if constexpr (kCtas > 1) cluster.barrier_wait();  // no CTA ends while another may read its memory
 }
 
 __global__ void __launch_bounds__(kCopyWarps * 32) splitd_evict_copy_kernel(const __grid_constant__ EvictParams p) {
@@ -224,7 +224,9 @@ __global__ void __launch_bounds__(kCopyWarps * 32) splitd_evict_copy_kernel(cons
   const int place = blockIdx.x * (kCopyWarps / 2) + (warp >> 1);
   pdl_wait();
   if (place >= p.keep) return;
-  const int slot = p.kept[static_cast<int64_t>(b) * p.keep + place];
+  const int64_t at = static_cast<int64_t>(b) * p.keep + place;
+  const int slot = p.kept[at];
+  if (lane == 0 && (warp & 1) == 0) p.new_weights[at] = slot < 0 ? 0.f : __ldg(p.weights + b * p.weights_stride + slot);
   if (slot < 0) return;
   int entry, row_from, row_to;
   split_slot(p.from, slot, entry, row_from);

@@ -219,10 +219,10 @@ def test_evict_longer_than_the_keys_in_shared_memory(kind):
     """More than 8 x 49152 slots; page table entries all name the same few pages (reading shared pages is fine)."""
     from splitd_flash_attn import split_paged_evict_func
 
-    n, keep = 500001, 1003
+    n, keep = 800001, 1003
     k = torch.randn(10, 1000, 1, D, device="cuda").to(torch.bfloat16)
     v = torch.randn(10, 1000, 1, D, device="cuda").to(torch.bfloat16)
-    table = (torch.arange(501, device="cuda", dtype=torch.int32) % 8)[None]
+    table = (torch.arange(801, device="cuda", dtype=torch.int32) % 8)[None]
     new = torch.tensor([[8, 9]], device="cuda", dtype=torch.int32)
     w = some_weights([n], kind, 5)
     m, kept, nw = split_paged_evict_func(k, v, table, torch.tensor([n], device="cuda", dtype=torch.int32), w, new, keep, 1, 2)
