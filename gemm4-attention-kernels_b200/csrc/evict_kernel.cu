@@ -63,8 +63,8 @@ __device__ __forceinline__ uint32_t order_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ int cache_len(const EvictParams& p, int b) {
-  return min(min(max(__ldg(p.seqlens + b), 0), page_capacity(p.from)), p.weights_len);
+__device__ __forceinline__ int cache_len(const EvictParams& p, int len) {
+  return min(min(max(len, 0), page_capacity(p.from)), p.weights_len);
 }
 
 template <int kCtas>
@@ -82,11 +82,23 @@ __global__ void __launch_bounds__(kThreads) splitd_evict_select_kernel(const __g
   const int b = blockIdx.x / kCtas, rank = kCtas > 1 ? static_cast<int>(cluster.block_rank()) : 0;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int gtid = rank * kThreads + tid, step = kCtas * kThreads;
-  const int n = cache_len(p, b);
+  // One thread of the cluster reads the length: threads that saw different ones would wait for each other for good.
+  __shared__ int length[2];
+  if (gtid == 0) length[0] = __ldg(p.seqlens + b), length[1] = cache_len(p, length[0]);
+  int n = 0, stated = 0;
+  if constexpr (kCtas > 1) {
+    cluster.sync();
+    const int* first = cluster.map_shared_rank(length, 0);
+    stated = first[0], n = first[1];
+    cluster.sync();  // no CTA ends while another may read its memory
+  } else {
+    __syncthreads();
+    stated = length[0], n = length[1];
+  }
   const int m = min(n, p.keep);
   if (gtid == 0) {
     p.new_seqlens[b] = m;
-    if (p.status && __ldg(p.seqlens + b) > n) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
+    if (p.status && stated > n) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
   }
   int* kept = p.kept + static_cast<int64_t>(b) * p.keep;
   for (int i = m + gtid; i < p.keep; i += step) kept[i] = -1;

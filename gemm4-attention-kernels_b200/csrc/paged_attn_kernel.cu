@@ -14,7 +14,7 @@
 // Split. The (sequence, KV head, row block) units are laid end to end, in tiles of 32 keys, and every CTA takes an
 // equal share of the whole line, whatever the lengths are; the lengths never leave the device. A unit that lies inside
 // one CTA is finished there. Each CTA has at most two unfinished ones (its first and its last), whose (m, l, O) go to
-// the workspace in fp32, and the join kernel adds them up in CTA order: no atomics, the same bits every time.
+// the workspace in fp32, and a second kernel adds them up in CTA order: no atomics, the same bits every time.
 //
 // Products. keys x rows on the warp matrix instruction (16 keys x 8 rows x 16): the cache row is the A operand, so a
 // group of 8 query heads fills the 8 columns exactly. S^T = K Q^T is split over two key halves and four quarters of
@@ -96,7 +96,7 @@ struct PagedAttnParams {
   // workspace
   float* part_o;   // [CTA][2][rows_per_block][512]
   float2* part_ml; // [CTA][2][rows_per_block]
-  float* lse2;     // [batch][heads_kv * rows] in log2 units, only with key_weights
+  float* lse2;     // [batch][heads_kv * rows] in log2 units, of the rows that one CTA finished; only with key_weights
   float* scores;   // [batch][heads_kv * rows][weights_len], only with key_weights
   float* weights;
   int64_t weights_stride;
@@ -405,6 +405,13 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
     }
     __syncwarp();
 
+    // with key_weights: where the scores of this warp's rows go, and how many of their keys are counted
+    const int n_rows = min(p.rows_per_block, p.rows - d.row0);
+    const int counted = p.scores ? min(d.len, p.weights_len) : 0;
+    const int64_t score_pitch = static_cast<int64_t>(8) * p.weights_len;
+    float* const score_row =
+        p.scores + (static_cast<int64_t>(d.b) * p.heads_kv * p.rows + d.head * p.rows + d.row0 + warp) * p.weights_len;
+
     // partial scores of the tile in the ring's next stage: 16 keys x rows over a quarter of the head dimension
     float s[kNB][4];
     auto scores = [&]() {
@@ -455,11 +462,11 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
         if (key < vis.x || key >= vis.y) x[k] = -INFINITY;
         top[k] = warp_max(x[k]);
       }
-      if (p.scores) {
+      if (key < counted) {
+        float* to = score_row + key;
 #pragma unroll
         for (int k = 0; k < kNB; ++k)
-          if (key < d.len && key < p.weights_len && bounds[warp + 8 * k].y > 0)
-            p.scores[(static_cast<int64_t>(d.b) * p.heads_kv * p.rows + d.head * p.rows + d.row0 + warp + 8 * k) * p.weights_len + key] = x[k];
+          if (warp + 8 * k < n_rows) to[k * score_pitch] = x[k];
       }
 #pragma unroll
       for (int k = 0; k < kNB; ++k) {
@@ -614,63 +621,61 @@ __global__ void __launch_bounds__(kThreads, 1) splitd_paged_attn_kernel(const __
   }
 }
 
+// How the line of tiles falls on one sequence, from the lengths alone. One warp.
+struct Span {
+  long long total, first;  // tiles of all sequences, and before this one
+  int n_tiles, len;        // tiles of a unit of this sequence
+};
+__device__ __forceinline__ Span span_of(const PagedAttnParams& p, int b, int lane) {
+  long long before = 0, after = 0;
+  Span s;
+  s.n_tiles = 0, s.len = 0;
+  for (int i = lane; i < p.batch; i += 32) {
+    const int len = seq_len(p, i), t = seq_tiles(p, len);
+    if (i < b) before += t; else after += t;
+    if (i == b) s.n_tiles = t, s.len = len;
+  }
+  const int units = p.heads_kv * p.row_blocks;
+  s.first = warp_sum(before) * units, s.total = s.first + warp_sum(after) * units;
+  s.n_tiles = __shfl_sync(0xffffffffu, s.n_tiles, b & 31), s.len = __shfl_sync(0xffffffffu, s.len, b & 31);
+  return s;
+}
+// The CTAs [first, last] whose shares hold parts of a unit.
+__device__ __forceinline__ int2 owners(const PagedAttnParams& p, const Span& s, int unit) {
+  const Line line = make_line(p, s.total);
+  const long long t0 = s.first + static_cast<long long>(unit) * s.n_tiles;
+  return make_int2(line.owner(t0), line.owner(t0 + s.n_tiles - 1));
+}
+// Partial result of CTA c: the first owner's share ends inside the unit (its second one); the others begin inside it.
+__device__ __forceinline__ int slot_of(int c, int first) { return c == first ? 2 * c + 1 : 2 * c; }
+
 // One block per output row: adds up the partial results of the CTAs that share the row's unit, or writes the row of a
 // sequence without keys. Rows whose unit lay inside one CTA are finished already. kGroups groups of kCols / 4 threads, 4
-// columns each; group g takes every kGroups-th partial result; blockIdx.z counts slices of kCols columns.
+// columns each; group g takes every kGroups-th partial result; `slice` counts the kCols columns of this block.
 template <bool kFp16, int kGroups, int kCols>
-__global__ void __launch_bounds__(kGroups * kCols / 4) splitd_paged_join_kernel(const __grid_constant__ PagedAttnParams p) {
+__device__ __forceinline__ void join_row(const PagedAttnParams& p, const Span& span, int b, int hr, int slice) {
   constexpr int kPer = kCols / 4;  // threads of a group
   __shared__ float4 acc[kGroups][kGroups > 1 ? kPer : 1];
-  const int col0 = blockIdx.z * kCols;
-  __shared__ long long span[3];  // line total, first tile of this sequence, tiles of a unit of it
-  pdl_launch_dependents();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int hr = blockIdx.x, b = blockIdx.y;  // hr = head * rows + row of the unit's KV head
+  const int tid = threadIdx.x, lane = tid & 31, col0 = slice * kCols;
   const int head = hr / p.rows, unit_row = hr - head * p.rows;
   const int rb = unit_row / p.rows_per_block, row = unit_row - rb * p.rows_per_block;
-  const int units = p.heads_kv * p.row_blocks;
-  if (hr == 0 && tid == 0 && __ldg(p.seqlens + b) > page_capacity(p.map) && p.status) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
-  if (warp == 0) {
-    long long before = 0, after = 0;
-    int mine = 0;
-    for (int i = lane; i < p.batch; i += 32) {
-      const int t = seq_tiles(p, seq_len(p, i));
-      if (i < b) before += t; else after += t;
-      if (i == b) mine = t;
-    }
-    before = warp_sum(before) * units, after = warp_sum(after) * units;
-    mine = __shfl_sync(0xffffffffu, mine, b & 31);
-    if (lane == 0) span[0] = before + after, span[1] = before, span[2] = mine;
-  }
-  __syncthreads();
-  const int n_tiles = static_cast<int>(span[2]);
   const int i = unit_row / p.group, g = unit_row - i * p.group;
   const int hq = head * p.group + g;
   uint16_t* out = p.o + b * p.o_sb + i * p.o_ss + hq * p.o_sh;
   const int64_t lse_at = (static_cast<int64_t>(b) * p.heads_q + hq) * p.sq + i;
-  const int64_t lse2_at = static_cast<int64_t>(b) * p.heads_kv * p.rows + hr;
-  int c0 = 0, c1 = -1;
-  if (n_tiles > 0) {
-    const Line line = make_line(p, span[0]);
-    const long long t0 = span[1] + static_cast<long long>(head * p.row_blocks + rb) * n_tiles;
-    c0 = line.owner(t0), c1 = line.owner(t0 + n_tiles - 1);
-  }
+  const int2 own = span.n_tiles > 0 ? owners(p, span, head * p.row_blocks + rb) : make_int2(0, -1);
   pdl_wait();
-  if (n_tiles == 0) {
+  if (span.n_tiles == 0) {
     if (tid < kCols / 8) *reinterpret_cast<uint4*>(out + col0 + tid * 8) = make_uint4(0, 0, 0, 0);
-    if (tid == 0 && col0 == 0) {
-      if (p.lse) p.lse[lse_at] = -INFINITY;
-      if (p.lse2) p.lse2[lse2_at] = -INFINITY;
-    }
+    if (tid == 0 && col0 == 0 && p.lse) p.lse[lse_at] = -INFINITY;
     return;
   }
-  if (c0 == c1) return;
-  // the first CTA's share ends inside the unit (its second partial result); all later CTAs begin inside the unit
-  auto slot_of = [&](int c) { return c == c0 ? 2 * c + 1 : 2 * c; };
-  auto ml_of = [&](int c) { return p.part_ml[slot_of(c) * p.rows_per_block + row]; };
-  float2 ml = c0 + lane <= c1 ? ml_of(c0 + lane) : make_float2(-INFINITY, 0.f);
+  if (own.x == own.y) return;
+  auto ml_of = [&](int c) { return p.part_ml[slot_of(c, own.x) * p.rows_per_block + row]; };
+  const float2 none = make_float2(-INFINITY, 0.f);
+  float2 ml = own.x + lane <= own.y ? ml_of(own.x + lane) : none;
   float m = ml.x;
-  for (int c = c0 + 32 + lane; c <= c1; c += 32) m = fmaxf(m, ml_of(c).x);
+  for (int c = own.x + 32 + lane; c <= own.y; c += 32) m = fmaxf(m, ml_of(c).x);
   m = warp_max(m);
   const float ref = m == -INFINITY ? 0.f : m;
   const int grp = tid / kPer, col = col0 + tid % kPer * 4;
@@ -678,14 +683,14 @@ __global__ void __launch_bounds__(kGroups * kCols / 4) splitd_paged_join_kernel(
   const int64_t pitch = static_cast<int64_t>(p.rows_per_block) * kHeadDim;
   float l = 0.f;
   float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int cc = c0; cc <= c1; cc += 32) {  // lane: weight of partial result cc + lane
-    if (cc > c0) ml = cc + lane <= c1 ? ml_of(cc + lane) : make_float2(-INFINITY, 0.f);
+  for (int cc = own.x; cc <= own.y; cc += 32) {  // lane: weight of partial result cc + lane
+    if (cc > own.x) ml = cc + lane <= own.y ? ml_of(cc + lane) : none;
     const float w = ex2(ml.x - ref);
     l += w * ml.y;
-    const int n = min(32, c1 - cc + 1);
+    const int n = min(32, own.y - cc + 1);
 #pragma unroll 4
     for (int k = grp; k < n; k += kGroups) {
-      const float4 v = __ldcs(reinterpret_cast<const float4*>(base + slot_of(cc + k) * pitch));
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(base + slot_of(cc + k, own.x) * pitch));
       const float wk = __shfl_sync(0xffffffffu, w, k);
       s.x += wk * v.x, s.y += wk * v.y, s.z += wk * v.z, s.w += wk * v.w;
     }
@@ -706,34 +711,91 @@ __global__ void __launch_bounds__(kGroups * kCols / 4) splitd_paged_join_kernel(
   uint2 w;
   w.x = pack2<kFp16>(s.x * inv, s.y * inv), w.y = pack2<kFp16>(s.z * inv, s.w * inv);
   *reinterpret_cast<uint2*>(out + col) = w;
-  if (tid == 0 && col0 == 0) {
-    const float l2 = l == 0.f ? -INFINITY : m + log2f(l);
-    if (p.lse) p.lse[lse_at] = l2 * kLn2;
-    if (p.lse2) p.lse2[lse2_at] = l2;
-  }
+  if (tid == 0 && col0 == 0 && p.lse) p.lse[lse_at] = (l == 0.f ? -INFINITY : m + log2f(l)) * kLn2;
 }
 
-constexpr int kWeightThreads = 256;
-
-// key_weights[b][j] += sum over the query rows of 2^(x - lse2), in row order. One key per thread.
-__global__ void __launch_bounds__(kWeightThreads) splitd_paged_weights_kernel(const __grid_constant__ PagedAttnParams p) {
-  const int b = blockIdx.y;
-  const int len = seq_len(p, b);
-  if (blockIdx.x == 0 && threadIdx.x == 0 && len > p.weights_len && p.status) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
-  const int n = min(len, p.weights_len);
-  const int key = first_key(p, len) + blockIdx.x * kWeightThreads + threadIdx.x;
-  pdl_wait();
-  if (key >= n) return;
+// key_weights[b][key] += sum over the query rows of 2^(x - lse2), in row order; one key per thread. The lse of a row is
+// formed here once more from the partial (m, l), so that this does not have to wait for the join: by one thread per row,
+// or by one warp where many CTAs share a unit (kWide).
+template <int kThreads, bool kWide>
+__device__ __forceinline__ void add_weights(const PagedAttnParams& p, const Span& span, int b, int block) {
+  constexpr int kRows = kWide ? 64 : kThreads;  // rows at a time
+  __shared__ float lse2[kRows];
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int n = min(span.len, p.weights_len);
+  const int key0 = first_key(p, span.len) + block * kThreads;
   const int rows = p.heads_kv * p.rows;
-  const float* x = p.scores + static_cast<int64_t>(b) * rows * p.weights_len + key;
-  const float* l2 = p.lse2 + static_cast<int64_t>(b) * rows;
-  float sum = 0.f;
-#pragma unroll 8
-  for (int r = 0; r < rows; ++r) {
-    const float l = __ldg(l2 + r), v = __ldcs(x + static_cast<int64_t>(r) * p.weights_len);
-    sum += l == -INFINITY ? 0.f : ex2(v - l);
+  if (block == 0 && tid == 0 && span.len > p.weights_len && p.status) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
+  if (key0 >= n) {
+    pdl_wait();
+    return;
   }
-  p.weights[b * p.weights_stride + key] += sum;
+  const int key = key0 + tid;
+  const float* x = p.scores + static_cast<int64_t>(b) * rows * p.weights_len + key;
+  float sum = 0.f;
+  for (int r0 = 0; r0 < rows; r0 += kRows) {
+    const int nr = min(kRows, rows - r0);
+    if (r0 > 0) __syncthreads();
+    for (int r = kWide ? tid >> 5 : tid; r < nr; r += kWide ? kThreads / 32 : kThreads) {
+      const int hr = r0 + r;
+      const int head = hr / p.rows, unit_row = hr - head * p.rows;
+      const int rb = unit_row / p.rows_per_block, row = unit_row - rb * p.rows_per_block;
+      const int2 own = owners(p, span, head * p.row_blocks + rb);
+      if (r0 == 0 && r == (kWide ? tid >> 5 : tid)) pdl_wait();
+      float m = -INFINITY, l = 0.f;
+      if (own.x == own.y) {
+        m = p.lse2[static_cast<int64_t>(b) * rows + hr], l = 1.f;
+      } else {
+#pragma unroll 4
+        for (int c = kWide ? own.x + lane : own.x; c <= own.y; c += kWide ? 32 : 1) {
+          const float2 ml = p.part_ml[slot_of(c, own.x) * p.rows_per_block + row];
+          const float top = fmaxf(m, ml.x), ref = top == -INFINITY ? 0.f : top;
+          l = l * ex2(m - ref) + ml.y * ex2(ml.x - ref);
+          m = top;
+        }
+        if constexpr (kWide) {
+          const float top = warp_max(m), ref = top == -INFINITY ? 0.f : top;
+          l *= ex2(m - ref);
+#pragma unroll
+          for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+          m = top;
+        }
+      }
+      if (!kWide || lane == 0) lse2[r] = l == 0.f ? -INFINITY : m + log2f(l);
+    }
+    if (r0 == 0) pdl_wait();
+    __syncthreads();
+    if (key < n) {
+#pragma unroll 16
+      for (int r = 0; r < nr; ++r) {
+        const float l2 = lse2[r], v = __ldcs(x + static_cast<int64_t>(r0 + r) * p.weights_len);
+        sum += l2 == -INFINITY ? 0.f : ex2(v - l2);
+      }
+    }
+  }
+  if (key < n) p.weights[b * p.weights_stride + key] += sum;
+}
+
+// What is left when all shares are done: blockIdx.y is the sequence; the first heads_kv * rows * (512 / kCols) blocks join
+// a row (or a slice of it) each, the others (with key_weights) add up the weights of kGroups * kCols / 4 keys each.
+template <bool kFp16, int kGroups, int kCols>
+__global__ void __launch_bounds__(kGroups * kCols / 4) splitd_paged_finish_kernel(const __grid_constant__ PagedAttnParams p) {
+  constexpr int kSlices = kHeadDim / kCols;
+  __shared__ Span shared_span;
+  const int b = blockIdx.y, n_join = p.heads_kv * p.rows * kSlices;
+  if (threadIdx.x < 32) {
+    const Span s = span_of(p, b, threadIdx.x);
+    if (threadIdx.x == 0) shared_span = s;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0 && __ldg(p.seqlens + b) > page_capacity(p.map) && p.status)
+    atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
+  __syncthreads();
+  const Span span = shared_span;
+  const int block = blockIdx.x;
+  if (block < n_join)
+    join_row<kFp16, kGroups, kCols>(p, span, b, block / kSlices, block % kSlices);
+  else
+    add_weights<kGroups * kCols / 4, (kGroups > 1)>(p, span, b, block - n_join);
 }
 
 }  // namespace pa
@@ -862,23 +924,21 @@ int launch_paged_attn(const splitd_paged_params* a, cudaStream_t stream) {
     e = fp16 ? launch_main<true, 4>(p, grid, stream) : launch_main<false, 4>(p, grid, stream);
   if (e) return e;
   cudaError_t ce = cudaGetLastError();
-  if (ce == cudaSuccess) {
-    // Few units: many CTAs share one, and sixteen groups of threads read their partial results side by side (1 x 131072
-    // keys, 37 results a row: 7 us with four groups, 4 with sixteen).
-    // The choice, which decides the order of the sums, does not look at the width of the page table.
-    const unsigned rows = p.heads_kv * p.rows;
-    if (static_cast<int64_t>(p.batch) * p.heads_kv * p.row_blocks * 8 <= sm_count())
-      ce = launch_dependent(fp16 ? pa::splitd_paged_join_kernel<true, 16, 128> : pa::splitd_paged_join_kernel<false, 16, 128>,
-                            dim3(rows, p.batch, 4), dim3(512), 0, stream, p);
-    else
-      ce = launch_dependent(fp16 ? pa::splitd_paged_join_kernel<true, 1, 512> : pa::splitd_paged_join_kernel<false, 1, 512>,
-                            dim3(rows, p.batch), dim3(128), 0, stream, p);
-  }
-  if (ce == cudaSuccess && p.weights) {
-    const int64_t longest = max_keys(a) < p.weights_len ? max_keys(a) : p.weights_len;
-    ce = launch_dependent(pa::splitd_paged_weights_kernel,
-                          dim3(static_cast<unsigned>((longest + pa::kWeightThreads - 1) / pa::kWeightThreads), p.batch),
-                          dim3(pa::kWeightThreads), 0, stream, p);
+  // Few units: many CTAs share one, and sixteen groups of threads read their partial results side by side (1 x 131072
+  // keys, 37 results a row: 7 us with four groups, 4 with sixteen). The choice, which decides the order of the sums, does
+  // not look at the width of the page table.
+  const bool few = static_cast<int64_t>(p.batch) * p.heads_kv * p.row_blocks * 8 <= sm_count();
+  const int64_t longest = !p.weights ? 0 : max_keys(a) < p.weights_len ? max_keys(a) : p.weights_len;
+  const unsigned rows = p.heads_kv * p.rows;
+  if (ce != cudaSuccess) {
+  } else if (few) {
+    const dim3 blocks(rows * 4 + static_cast<unsigned>((longest + 511) / 512), p.batch);
+    ce = launch_dependent(fp16 ? pa::splitd_paged_finish_kernel<true, 16, 128> : pa::splitd_paged_finish_kernel<false, 16, 128>, blocks,
+                          dim3(512), 0, stream, p);
+  } else {
+    const dim3 blocks(rows + static_cast<unsigned>((longest + 127) / 128), p.batch);
+    ce = launch_dependent(fp16 ? pa::splitd_paged_finish_kernel<true, 1, 512> : pa::splitd_paged_finish_kernel<false, 1, 512>, blocks,
+                          dim3(128), 0, stream, p);
   }
   if (ce != cudaSuccess) {
     cudaGetLastError();
