@@ -71,6 +71,21 @@ int check_common(const splitd_params* p, bool backward);
 int check_device();
 void clear_error();
 
+// SMs of the current device (asked for once per device)
+inline int sm_count() {
+  static std::atomic<int> cache[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64) {
+    const int c = cache[dev].load(std::memory_order_acquire);
+    if (c > 0) return c;
+  }
+  int n = 0;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  if (dev >= 0 && dev < 64) cache[dev].store(n, std::memory_order_release);
+  return n;
+}
+
 // Number of 2-CTA clusters of `kern` the current device keeps resident at once (the grid of a persistent
 // kernel). `cache` holds one entry per device index and is filled on first use, which is also where the kernel's
 // dynamic shared memory limit is raised (once per device instead of once per launch). Concurrent first calls

@@ -807,20 +807,6 @@ int rows_per_block_of(int rows) { return (rows + row_blocks_of(rows) - 1) / row_
 
 int64_t max_keys(const splitd_paged_params* p) { return static_cast<int64_t>(p->max_pages) * p->page_size; }
 
-int sm_count() {
-  static std::atomic<int> cache[64];
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev >= 0 && dev < 64) {
-    const int c = cache[dev].load(std::memory_order_acquire);
-    if (c > 0) return c;
-  }
-  int n = 0;
-  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
-  if (dev >= 0 && dev < 64) cache[dev].store(n, std::memory_order_release);
-  return n;
-}
-
 constexpr int kMinTiles = 1;
 constexpr int kMaxCtas = 256;  // sizes the workspace without asking a device
 
@@ -924,10 +910,11 @@ int launch_paged_attn(const splitd_paged_params* a, cudaStream_t stream) {
     e = fp16 ? launch_main<true, 4>(p, grid, stream) : launch_main<false, 4>(p, grid, stream);
   if (e) return e;
   cudaError_t ce = cudaGetLastError();
-  // Few units: many CTAs share one, and sixteen groups of threads read their partial results side by side (1 x 131072
-  // keys, 37 results a row: 7 us with four groups, 4 with sixteen). The choice, which decides the order of the sums, does
-  // not look at the width of the page table.
-  const bool few = static_cast<int64_t>(p.batch) * p.heads_kv * p.row_blocks * 8 <= sm_count();
+  // Few rows (so few units, each shared by many CTAs): four blocks a row, in which sixteen groups of threads read partial
+  // results side by side (1 x 131072 keys, 32 rows, 37 results each: 4 us, 7 us with one block of four groups a row). More
+  // rows: one small block each (8 x 230 keys, 512 rows, 8 results each: ... us, 19 us the other way). The choice, which
+  // decides the order of the sums, does not look at the width of the page table.
+  const bool few = static_cast<int64_t>(p.batch) * p.heads_kv * p.rows <= sm_count();
   const int64_t longest = !p.weights ? 0 : max_keys(a) < p.weights_len ? max_keys(a) : p.weights_len;
   const unsigned rows = p.heads_kv * p.rows;
   if (ce != cudaSuccess) {

@@ -78,8 +78,8 @@ __device__ __forceinline__ int sequence_of(const int* cu, int batch, int t, int 
   return -1;
 }
 
-template <bool kFp16, int kLayout>
-__global__ void __launch_bounds__(kWarps * 32) splitd_rotary_kernel(const __grid_constant__ RotaryParams p) {
+template <bool kFp16, int kLayout, int kBlocksPerSm>
+__global__ void __launch_bounds__(kWarps * 32, kBlocksPerSm) splitd_rotary_kernel(const __grid_constant__ RotaryParams p) {
   __shared__ __align__(16) uint16_t stage[kLayout == kHalfOdd ? kWarps : 1][kLayout == kHalfOdd ? kHeadDim : 8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t work = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
@@ -246,35 +246,49 @@ __global__ void __launch_bounds__(kWarps * 32) splitd_rotary_kernel(const __grid
 
 namespace {
 
+template <bool kFp16, int kLayout>
+void launch_layout(const RotaryParams& p, unsigned blocks, cudaStream_t stream) {
+  if (blocks <= 2 * 148)
+    rot::splitd_rotary_kernel<kFp16, kLayout, 2><<<blocks, rot::kWarps * 32, 0, stream>>>(p);
+  else
+    rot::splitd_rotary_kernel<kFp16, kLayout, 3><<<blocks, rot::kWarps * 32, 0, stream>>>(p);
+}
+template <int kLayout>
+void launch_type(const RotaryParams& p, bool fp16, unsigned blocks, cudaStream_t stream) {
+  if (fp16)
+    launch_layout<true, kLayout>(p, blocks, stream);
+  else
+    launch_layout<false, kLayout>(p, blocks, stream);
+}
+
 int launch_rotary_kernel(RotaryParams& p, bool fp16, bool interleaved, cudaStream_t stream) {
   const int heads = p.heads_q + p.heads_k + p.heads_v;
-  // Long calls: a warp takes all heads of a token and forms its angles once. Short calls: heads are spread over
-  // warps, four rows (one round of loads) at least, until there are enough warps to fill the GPU.
-  constexpr int64_t kFill = 148 * 32;
-  int64_t groups = (kFill + p.tokens - 1) / p.tokens;
-  const int64_t most = (heads + rot::kUnroll - 1) / rot::kUnroll;
-  if (groups > most) groups = most;
+  // Up to 20 heads per warp, in rounds of four and equal runs where the number of heads allows it: a warp's angles cost as
+  // much as five of its heads, and much longer runs leave a tail (37 x 46 tokens, 40 heads: 25 us with two runs, 33 us with
+  // three of 14, 34 us with ten of 4; 2 x 8192 tokens, 36 heads: 193 us with three runs, 201 us with two of 18). Shorter
+  // runs when there would not be half as many warps as the GPU holds (6 x 103 tokens, 36 heads: 11 us with three runs, 13
+  // us with two), but four heads, one round of loads, at least. Calls of up to one wave of blocks get the registers of two blocks per SM (64 tokens: 5.7 us, 6.5 us
+  // with three), longer ones three blocks (2 x 8192 tokens: 195 us, 201 us with two).
+  constexpr int64_t kHalfFull = 148 * 24 / 2;
+  int64_t groups = (heads + 19) / 20;
+  for (int64_t g = groups; g <= 2 * groups; ++g)
+    if (heads % (4 * g) == 0) {
+      groups = g;
+      break;
+    }
+  const int64_t fill = (kHalfFull + p.tokens - 1) / p.tokens, most = (heads + rot::kUnroll - 1) / rot::kUnroll;
+  if (groups < fill) groups = fill < most ? fill : most;
   p.heads_per_warp = static_cast<int>((heads + groups - 1) / groups);
   p.groups = (heads + p.heads_per_warp - 1) / p.heads_per_warp;
   const int64_t blocks = (p.tokens * p.groups + rot::kWarps - 1) / rot::kWarps;
   if (blocks > 0x7fffffff) return fail(SPLITD_ERR_INVALID_ARGUMENT, "too many tokens for one call");
-  const dim3 grid(static_cast<unsigned>(blocks)), block(rot::kWarps * 32);
-  if (interleaved) {
-    if (fp16)
-      rot::splitd_rotary_kernel<true, rot::kInterleaved><<<grid, block, 0, stream>>>(p);
-    else
-      rot::splitd_rotary_kernel<false, rot::kInterleaved><<<grid, block, 0, stream>>>(p);
-  } else if (p.pairs % 8 == 0) {
-    if (fp16)
-      rot::splitd_rotary_kernel<true, rot::kHalf><<<grid, block, 0, stream>>>(p);
-    else
-      rot::splitd_rotary_kernel<false, rot::kHalf><<<grid, block, 0, stream>>>(p);
-  } else {
-    if (fp16)
-      rot::splitd_rotary_kernel<true, rot::kHalfOdd><<<grid, block, 0, stream>>>(p);
-    else
-      rot::splitd_rotary_kernel<false, rot::kHalfOdd><<<grid, block, 0, stream>>>(p);
-  }
+  const unsigned n = static_cast<unsigned>(blocks);
+  if (interleaved)
+    launch_type<rot::kInterleaved>(p, fp16, n, stream);
+  else if (p.pairs % 8 == 0)
+    launch_type<rot::kHalf>(p, fp16, n, stream);
+  else
+    launch_type<rot::kHalfOdd>(p, fp16, n, stream);
   const cudaError_t ce = cudaGetLastError();
   if (ce != cudaSuccess) return fail(SPLITD_ERR_CUDA, "rotary: launch failed: %s", cudaGetErrorString(ce));
   return 0;
