@@ -6,10 +6,14 @@
 // seen so far; two such triples of disjoint key sets join to one by scaling both to the larger m. o = O / l and
 // lse = (m + log2 l) ln 2; a row that sees no key has l = 0: o = 0, lse = -inf.
 //
-// What bounds it. Every visible key costs 2 KB of cache and 4 * 512 * R flops: at R = 8, 8 flops a byte, far left of
-// the ridge. So the kernel is built around the stream of cache rows: one CTA per SM, a producer warp that keeps a ring
-// of six 32-row stages (200 KB) full with one 1 KB bulk copy per row (a page of any size and a row of any page is
-// then the same thing: no tile has to match a page), and eight warps that have about four times the time they need.
+// What bounds it. Every visible key costs 2 KB of cache and 4 * 512 * R flops: at R = 8, 8 flops a byte, far left of the
+// ridge. So the kernel is built around the stream of cache rows: one CTA per SM, four producer warps that keep a ring of
+// 32-row stages full with one 1 KB bulk copy per row (a page of any size and a row of any page are then the same thing:
+// no tile has to match a page), and eight warps that compute. One producer warp alone can issue such a copy every 74
+// cycles, 59 % of the bandwidth. Measured: 1 x 131072 keys, 4 KV heads, 8 rows each: 158 us, 6.8 TB/s; 32 sequences of up
+// to 8192: 206 us, 6.8 TB/s (a plain copy moves 6.6). With 32 rows (4 tokens) a tile's instructions are what bounds it:
+// two computing warps per scheduler wait out their fixed latencies (tensor pipe 42 %, issue slots 40 %), 119 us where
+// the stream alone takes 94.
 //
 // Split. The (sequence, KV head, row block) units are laid end to end, in tiles of 32 keys, and every CTA takes an
 // equal share of the whole line, whatever the lengths are; the lengths never leave the device. A unit that lies inside
@@ -34,17 +38,18 @@ namespace pa {
 constexpr int kTile = 32;                      // keys per tile = rows per ring stage
 constexpr int kPitch = kRowBytes + 16;         // ldmatrix reads 8 rows at once: 16 bytes of padding spread them over the banks
 constexpr int kStageBytes = kTile * kPitch;
-constexpr int kConsumers = 256;                // threads of the eight warps that compute
+constexpr int kWarps = 8;                      // warps that compute
 constexpr int kProducers = 4;                  // producer warps: each asks for a quarter of a tile's rows
 constexpr int kRowsPerProducer = kTile / kProducers;
-constexpr int kThreads = kConsumers + 32 * kProducers;
+constexpr int kThreads = 32 * (kWarps + kProducers);
 constexpr int kPartPitch = 36;                 // floats per row of the partial scores (32 keys + padding)
 constexpr int kPPitch = 20;                    // 32-bit words per row of P (32 keys x 2 bytes + padding)
 constexpr int kMaxRows = 32;                   // rows of a row block
 
-// From 17 rows on a consumer thread needs more than the 168 registers that 384 threads can have each, so the producers
+// From 17 rows on a computing thread needs more than the 168 registers that 384 threads can have each, so the producers
 // give up some of theirs (4 tokens, 32 rows: 305 us with spills, 159 us with the split; with 8 rows the split costs 1 %).
-// The launch checks that the block comes with at least as many as the two shares together.
+// The launch checks that the block comes with at least as many as the two shares together. Sixteen computing warps were
+// tried instead: no faster with 16 rows, and 155 against 119 us with 32, where they read every row twice.
 template <int kNB>
 constexpr bool kSplitRegs = kNB >= 3;
 constexpr int kProducerRegs = 56, kConsumerRegs = 216;
@@ -62,8 +67,10 @@ struct Layout {
   // two of each of these: one tile's are read while the next one's are written
   static constexpr int kPartFloats = 4 * kRows * kPartPitch;
   static constexpr int kPWords = kRows * kPPitch;  // of each half of P
-  // as many stages as fit beside them; four in flight are enough to cover the latency of HBM
-  static constexpr int kStages = kNB <= 2 ? 6 : 5;
+  // Enough stages in flight to cover the latency of HBM, and no more: six would fit beside 8 rows, but the deeper queue of
+  // requests costs HBM efficiency (1 x 131072 keys: 172 us with six, 168 with five, 159 with four, 160 with three;
+  // 32 sequences up to 8192: 222, 215, 208, 210). With 32 rows a stage is held longer (119 us with five, 125 with four).
+  static constexpr int kStages = kNB <= 2 ? 4 : 5;
   static constexpr int kOffPart = kStages * kStageBytes;
   static constexpr int kOffP = kOffPart + 2 * kPartFloats * 4;
   static constexpr int kOffCorr = kOffP + 2 * 2 * kPWords * 4;
@@ -251,6 +258,11 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
           d.pad = 0;
           descs[r.stage] = d;
         }
+        if (active && my_row >= n_rows && my_row < L::kRows) {  // rows that pad the block: scores of 0, and no NaN
+          for (int c = 0; c < kRowBytes; c += 16) st_shared_v4(ring0 + r.stage * kStageBytes + my_row * kPitch + c, 0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
         if (lane == 0) mbar_arrive_expect_tx(bar, rows * kRowBytes);
         __syncwarp();
         if (active && my_row < n_rows) {
@@ -332,6 +344,9 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
                                          volatile int* abort_flag, int warp, int lane) {
   using L = Layout<kNB>;
   constexpr int kRows = L::kRows;
+  constexpr int kMT = kHeadDim / kWarps / 16;  // values: 16-column tiles of a warp
+  constexpr int kR = kRows / kWarps;           // softmax: rows of a warp (w, w + kWarps, ...)
+  static_assert(kWarps == 2 * 4, "scores: two key halves times four quarters of the head dimension");
   const Desc* descs = reinterpret_cast<const Desc*>(smem + L::kOffDesc);
   float* part0 = reinterpret_cast<float*>(smem + L::kOffPart);
   uint32_t* p0 = reinterpret_cast<uint32_t*>(smem + L::kOffP);
@@ -351,18 +366,18 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
     if (lane == 0) mbar_arrive(r.empty + 8 * r.stage);
     r.next();
   };
-  auto sync = [&]() { asm volatile("bar.sync 1, 256;" ::: "memory"); };
+  auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); };
 
   while (true) {
     bool ok = wait_full();
-    // All eight warps have to agree on whether to go on, or the ones that do would wait for the others for good.
+    // All of these warps have to agree on whether to go on, or the ones that do would wait for the others for good.
     int go;
     {
       const int mine = ok && !*abort_flag;
       asm volatile(
-          "{\n\t.reg .pred P, Q;\n\tsetp.ne.s32 P, %1, 0;\n\tbarrier.cta.red.and.pred Q, 1, 256, P;\n\tselp.s32 %0, 1, 0, Q;\n\t}"
+          "{\n\t.reg .pred P, Q;\n\tsetp.ne.s32 P, %1, 0;\n\tbarrier.cta.red.and.pred Q, 1, %2, P;\n\tselp.s32 %0, 1, 0, Q;\n\t}"
           : "=r"(go)
-          : "r"(mine)
+          : "r"(mine), "n"(32 * kWarps)
           : "memory");
     }
     if (!go) return;
@@ -382,33 +397,35 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
         }
     }
     release();
-    float o[4][kNB][4];
+    float o[kMT][kNB][4];
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
+    for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
       for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[mt][nb][e] = 0.f;
-    float m_row[kNB], l_row[kNB];
+    // Query token i sees the keys [i + see_lo, i + see_hi) of the sequence's [0, len).
+    const long long see_lo = p.win_left < 0 ? -(1ll << 40) : static_cast<long long>(d.len) - p.sq - p.win_left;
+    const long long see_hi = p.win_right < 0 ? 1ll << 40 : static_cast<long long>(d.len) - p.sq + p.win_right + 1;
+    const int n_rows = min(p.rows_per_block, p.rows - d.row0);
+    // keys that all rows of the block see: tiles inside need no mask
+    const int free_lo = static_cast<int>(max(0ll, (d.row0 + n_rows - 1) / p.group + see_lo));
+    const int free_hi = static_cast<int>(max(0ll, min(static_cast<long long>(d.len), d.row0 / p.group + see_hi)));
+    float m_row[kR], l_row[kR];
 #pragma unroll
-    for (int k = 0; k < kNB; ++k) {
+    for (int k = 0; k < kR; ++k) {
       m_row[k] = -INFINITY, l_row[k] = 0.f;
-      // keys [x, y) are visible to the row; only this warp reads its rows' bounds
-      const int row = d.row0 + warp + 8 * k;
-      int2 vis = make_int2(0, 0);
-      if (warp + 8 * k < p.rows_per_block && row < p.rows) {
-        const long long diag = static_cast<long long>(row / p.group) + d.len - p.sq;
-        vis.x = p.win_left < 0 ? 0 : static_cast<int>(max(0ll, diag - p.win_left));
-        vis.y = p.win_right < 0 ? d.len : static_cast<int>(max(0ll, min(static_cast<long long>(d.len), diag + p.win_right + 1)));
-      }
-      if (lane == 0) bounds[warp + 8 * k] = vis;
+      const int r = warp + kWarps * k, i = (d.row0 + r) / p.group;
+      if (lane == 0)  // only this warp reads its rows' bounds; rows that pad the block see nothing
+        bounds[r] = r < n_rows ? make_int2(static_cast<int>(max(0ll, i + see_lo)),
+                                           static_cast<int>(max(0ll, min(static_cast<long long>(d.len), i + see_hi))))
+                               : make_int2(0, 0);
     }
     __syncwarp();
 
     // with key_weights: where the scores of this warp's rows go, and how many of their keys are counted
-    const int n_rows = min(p.rows_per_block, p.rows - d.row0);
     const int counted = p.scores ? min(d.len, p.weights_len) : 0;
-    const int64_t score_pitch = static_cast<int64_t>(8) * p.weights_len;
+    const int64_t score_pitch = static_cast<int64_t>(kWarps) * p.weights_len;
     float* const score_row =
         p.scores + (static_cast<int64_t>(d.b) * p.heads_kv * p.rows + d.head * p.rows + d.row0 + warp) * p.weights_len;
 
@@ -437,40 +454,44 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
         dst[0] = s[nb][0], dst[kPartPitch] = s[nb][1], dst[8] = s[nb][2], dst[kPartPitch + 8] = s[nb][3];
       }
     };
-    // softmax: one row per warp (and n tile), one key per lane
+    // softmax: a row at a time per warp, one key per lane
     auto softmax = [&](int tile, int buf) {
       const int key = d.first_key + tile * kTile + lane;
       uint16_t* p_hi = reinterpret_cast<uint16_t*>(p0 + buf * 2 * L::kPWords);
       uint16_t* p_lo = p_hi + 2 * L::kPWords;
       // step by step over all rows, so that their latencies overlap
-      float x[kNB], top[kNB];
+      float x[kR], top[kR];
 #pragma unroll
-      for (int k = 0; k < kNB; ++k) {
-        const float* src = part0 + buf * L::kPartFloats + (warp + 8 * k) * kPartPitch + lane;
+      for (int k = 0; k < kR; ++k) {
+        const float* src = part0 + buf * L::kPartFloats + (warp + kWarps * k) * kPartPitch + lane;
         x[k] = (src[0] + src[kRows * kPartPitch]) + (src[2 * kRows * kPartPitch] + src[3 * kRows * kPartPitch]);
       }
       if (p.softcap > 0.f) {
 #pragma unroll
-        for (int k = 0; k < kNB; ++k) x[k] = cap_out * tanhf(x[k] * cap_in);
+        for (int k = 0; k < kR; ++k) x[k] = cap_out * tanhf(x[k] * cap_in);
       } else {
 #pragma unroll
-        for (int k = 0; k < kNB; ++k) x[k] *= scale_log2;
+        for (int k = 0; k < kR; ++k) x[k] *= scale_log2;
+      }
+      const int key0 = d.first_key + tile * kTile;
+      if (key0 < free_lo || key0 + kTile > free_hi) {
+#pragma unroll
+        for (int k = 0; k < kR; ++k) {
+          const int2 vis = bounds[warp + kWarps * k];
+          if (key < vis.x || key >= vis.y) x[k] = -INFINITY;
+        }
       }
 #pragma unroll
-      for (int k = 0; k < kNB; ++k) {
-        const int2 vis = bounds[warp + 8 * k];
-        if (key < vis.x || key >= vis.y) x[k] = -INFINITY;
-        top[k] = warp_max(x[k]);
-      }
+      for (int k = 0; k < kR; ++k) top[k] = warp_max(x[k]);
       if (key < counted) {
         float* to = score_row + key;
 #pragma unroll
-        for (int k = 0; k < kNB; ++k)
-          if (warp + 8 * k < n_rows) to[k * score_pitch] = x[k];
+        for (int k = 0; k < kR; ++k)
+          if (warp + kWarps * k < n_rows) to[k * score_pitch] = x[k];
       }
 #pragma unroll
-      for (int k = 0; k < kNB; ++k) {
-        const int row = warp + 8 * k;
+      for (int k = 0; k < kR; ++k) {
+        const int row = warp + kWarps * k;
         const float m_new = fmaxf(m_row[k], top[k]);
         // a row that has seen no key yet: any finite reference gives p = 0 (and NaN for scores that are NaN)
         const float ref = m_new == -INFINITY ? 0.f : m_new;
@@ -483,47 +504,43 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
         if (lane == 0) corr0[buf * kRows + row] = c;
       }
     };
-    // O^T += V^T P^T with the tile in the ring's next stage, 64 columns of the head dimension
+    // O^T += V^T P^T with the tile in the ring's next stage, a share of the head dimension's columns
     auto values = [&](int buf) {
       wait_full();
       const float* corr = corr0 + buf * kRows;
-      const uint32_t* pw_hi = p0 + buf * 2 * L::kPWords;
-      const uint32_t* pw_lo = pw_hi + L::kPWords;
-      float cf[kNB][2];
+      float2 cf[kNB];
       bool any = false;
 #pragma unroll
       for (int nb = 0; nb < kNB; ++nb) {
-        cf[nb][0] = corr[nb * 8 + frag_col], cf[nb][1] = corr[nb * 8 + frag_col + 1];
-        any |= cf[nb][0] != 1.f || cf[nb][1] != 1.f;
+        cf[nb] = *reinterpret_cast<const float2*>(corr + nb * 8 + frag_col);
+        any |= cf[nb].x != 1.f || cf[nb].y != 1.f;
       }
       if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
+        for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
           for (int nb = 0; nb < kNB; ++nb) {
-            o[mt][nb][0] *= cf[nb][0], o[mt][nb][1] *= cf[nb][1];
-            o[mt][nb][2] *= cf[nb][0], o[mt][nb][3] *= cf[nb][1];
+            o[mt][nb][0] *= cf[nb].x, o[mt][nb][1] *= cf[nb].y;
+            o[mt][nb][2] *= cf[nb].x, o[mt][nb][3] *= cf[nb].y;
           }
       }
       const uint32_t base =
-          ring0 + r.stage * kStageBytes + ((lane & 7) + (lane >> 4) * 8) * kPitch + warp * 128 + ((lane >> 3) & 1) * 16;
+          ring0 + r.stage * kStageBytes + ((lane & 7) + (lane >> 4) * 8) * kPitch + warp * (kMT * 32) + ((lane >> 3) & 1) * 16;
+      // P as B operand, one load per k step and n tile: its upper numbers' two registers, then its lower ones'
+      const uint32_t p_base = smem_u32(p0 + (buf * 2 + (lane >> 4)) * L::kPWords) + (lane & 7) * (kPPitch * 4) + ((lane >> 3) & 1) * 16;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        uint32_t bh[kNB][2], bl[kNB][2];
+        uint32_t a[kMT][4];
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt) ldmatrix_x4_trans(base + ks * 16 * kPitch + mt * 32, a[mt]);
 #pragma unroll
         for (int nb = 0; nb < kNB; ++nb) {
-          const int at = (nb * 8 + frag_row) * kPPitch + ks * 8 + (lane & 3);
-          bh[nb][0] = pw_hi[at], bh[nb][1] = pw_hi[at + 4];
-          bl[nb][0] = pw_lo[at], bl[nb][1] = pw_lo[at + 4];
-        }
+          uint32_t pf[4];
+          ldmatrix_x4(p_base + nb * 8 * kPPitch * 4 + ks * 32, pf);
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-          uint32_t a[4];
-          ldmatrix_x4_trans(base + ks * 16 * kPitch + mt * 32, a);
+          for (int mt = 0; mt < kMT; ++mt) mma_16816<kFp16>(o[mt][nb], a[mt], pf[0], pf[1]);
 #pragma unroll
-          for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(o[mt][nb], a, bh[nb][0], bh[nb][1]);
-#pragma unroll
-          for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(o[mt][nb], a, bl[nb][0], bl[nb][1]);
+          for (int mt = 0; mt < kMT; ++mt) mma_16816<kFp16>(o[mt][nb], a[mt], pf[2], pf[3]);
         }
       }
       release();
@@ -545,11 +562,11 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
     values((d.n_tiles - 1) & 1);
     // ---- the stretch is done
 #pragma unroll
-    for (int k = 0; k < kNB; ++k) {
+    for (int k = 0; k < kR; ++k) {
       float l = l_row[k];
 #pragma unroll
       for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
-      const int row = warp + 8 * k;
+      const int row = warp + kWarps * k;
       if (lane == 0) {
         stat[row] = make_float2(m_row[k], l);
         const int unit_row = d.row0 + row;
@@ -573,21 +590,21 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
         const int row = nb * 8 + frag_col + e;
         const int unit_row = d.row0 + row;
         if (row >= p.rows_per_block || unit_row >= p.rows) continue;
-        const int col = warp * 64 + frag_row;
+        const int col = warp * (kMT * 16) + frag_row;
         if (d.slot < 0) {
           const int i = unit_row / p.group, g = unit_row - i * p.group;
           const float l = stat[row].y;
           const float inv = l == 0.f ? 0.f : 1.f / l;
           uint16_t* dst = p.o + d.b * p.o_sb + i * p.o_ss + (d.head * p.group + g) * p.o_sh + col;
 #pragma unroll
-          for (int mt = 0; mt < 4; ++mt) {
+          for (int mt = 0; mt < kMT; ++mt) {
             dst[mt * 16] = static_cast<uint16_t>(pack2<kFp16>(o[mt][nb][e] * inv, 0.f) & 0xffffu);
             dst[mt * 16 + 8] = static_cast<uint16_t>(pack2<kFp16>(o[mt][nb][e + 2] * inv, 0.f) & 0xffffu);
           }
         } else {
           float* dst = p.part_o + (static_cast<int64_t>(blockIdx.x * 2 + d.slot) * p.rows_per_block + row) * kHeadDim + col;
 #pragma unroll
-          for (int mt = 0; mt < 4; ++mt) dst[mt * 16] = o[mt][nb][e], dst[mt * 16 + 8] = o[mt][nb][e + 2];
+          for (int mt = 0; mt < kMT; ++mt) dst[mt * 16] = o[mt][nb][e], dst[mt * 16 + 8] = o[mt][nb][e + 2];
         }
       }
   }
@@ -606,15 +623,15 @@ __global__ void __launch_bounds__(kThreads, 1) splitd_paged_attn_kernel(const __
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kStages; ++i) {
       mbar_init(r.full + 8 * i, kProducers);
-      mbar_init(r.empty + 8 * i, kConsumers / 32);
+      mbar_init(r.empty + 8 * i, kWarps);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
   __syncthreads();
-  if (warp >= kConsumers / 32) {
+  if (warp >= kWarps) {
     if constexpr (kSplitRegs<kNB>) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
-    producer<kNB>(p, smem, r, abort_flag, warp - kConsumers / 32, lane);
+    producer<kNB>(p, smem, r, abort_flag, warp - kWarps, lane);
   } else {
     if constexpr (kSplitRegs<kNB>) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
     consumer<kFp16, kNB>(p, smem, r, abort_flag, warp, lane);
@@ -829,7 +846,7 @@ size_t paged_workspace_bytes(const splitd_paged_params* p) {
 namespace {
 
 template <typename Kernel>
-int raise_smem(Kernel kern, int bytes, bool split_regs, std::atomic<int> (&done)[64]) {
+int raise_smem(Kernel kern, int bytes, int threads, bool split_regs, std::atomic<int> (&done)[64]) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire)) return 0;
@@ -840,7 +857,7 @@ int raise_smem(Kernel kern, int bytes, bool split_regs, std::atomic<int> (&done)
   if (split_regs) {
     cudaFuncAttributes at;
     if (cudaFuncGetAttributes(&at, kern) != cudaSuccess ||
-        at.numRegs * pa::kThreads < 32 * pa::kProducers * pa::kProducerRegs + pa::kConsumers * pa::kConsumerRegs) {
+        at.numRegs * threads < 32 * pa::kProducers * pa::kProducerRegs + (threads - 32 * pa::kProducers) * pa::kConsumerRegs) {
       cudaGetLastError();
       return fail(SPLITD_ERR_CUDA, "paged attention: built with too few registers for its split");
     }
@@ -853,7 +870,7 @@ template <bool kFp16, int kNB>
 int launch_main(const PagedAttnParams& p, int grid, cudaStream_t stream) {
   static std::atomic<int> done[64];
   auto kern = pa::splitd_paged_attn_kernel<kFp16, kNB>;
-  if (int e = raise_smem(kern, pa::Layout<kNB>::kBytes, pa::kSplitRegs<kNB>, done)) return e;
+  if (int e = raise_smem(kern, pa::Layout<kNB>::kBytes, pa::kThreads, pa::kSplitRegs<kNB>, done)) return e;
   kern<<<grid, pa::kThreads, pa::Layout<kNB>::kBytes, stream>>>(p);
   return 0;
 }
