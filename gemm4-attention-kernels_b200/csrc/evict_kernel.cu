@@ -11,11 +11,13 @@
 //
 // A cluster of eight CTAs per sequence, each with its share of the slots; histograms and counts meet through distributed
 // shared memory. Up to kOneCta slots a single CTA is faster than the cluster's barriers. The weights are read once and
-// their keys kept in shared memory (a sequence of more than eight times kCacheMost slots is read from L2 again). What bounds it is the chain of passes and barriers (131072 slots: 19 us;
-// the copy of 20000 of them, 4 heads: 50 us), not bytes.
+// their keys kept in shared memory (a sequence of more than eight times kCacheMost slots is read from L2 again). What
+// bounds it is the chain of passes and barriers (131072 slots: 19 us; the copy of 20000 of them, 4 heads: 50 us), not
+// bytes.
 //
-// Copy. One warp per kept slot and tensor, 16 bytes per lane, four head rows in flight; nothing is read or written
-// that does not move. It is bound by HBM: 2 * heads_kv KB read and written per slot.
+// Copy. The kept slots' head rows are laid end to end; a warp takes four of them of one tensor, whose places four of its
+// lanes look up side by side, and has all four in flight, 16 bytes per lane. Nothing is read or written that does not
+// move. It is bound by HBM: 2 * heads_kv KB read and written per slot.
 #include <cooperative_groups.h>
 
 #include <cstring>
@@ -31,10 +33,10 @@ constexpr int kCluster = 8;  // sixteen: the same time for one sequence of 13107
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kOneCta = 8192;
+constexpr int kOneCta = 16384;  // 8000 slots: 12 us, 14 us with the cluster; 16000: 17 us both ways; 32000: 27, 23
 constexpr int kCacheMost = 49152;  // keys that a CTA keeps in shared memory (192 KB)
 constexpr int kCopyWarps = 8;
-constexpr int kCopyUnroll = 4;
+constexpr int kCopyRows = 4;  // head rows of a warp
 }  // namespace ev
 
 struct EvictParams {
@@ -233,41 +235,49 @@ __global__ void __launch_bounds__(kThreads) splitd_evict_select_kernel(const __g
 __global__ void __launch_bounds__(kCopyWarps * 32) splitd_evict_copy_kernel(const __grid_constant__ EvictParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.y;
-  const int place = blockIdx.x * (kCopyWarps / 2) + (warp >> 1);
-  pdl_wait();
-  if (place >= p.keep) return;
-  const int64_t at = static_cast<int64_t>(b) * p.keep + place;
-  const int slot = p.kept[at];
-  if (lane == 0 && (warp & 1) == 0) p.new_weights[at] = slot < 0 ? 0.f : __ldg(p.weights + b * p.weights_stride + slot);
-  if (slot < 0) return;
-  int entry, row_from, row_to;
-  split_slot(p.from, slot, entry, row_from);
-  const int page_from = page_of(p.from, b, entry);
-  split_slot(p.to, place, entry, row_to);
-  const int page_to = page_of(p.to, b, entry);
-  if (!page_ok(p.from, page_from) || !page_ok(p.to, page_to)) {
-    if (lane == 0 && p.status) atomicCAS(p.status, 0, ST_BAD_PAGE);
-    return;
-  }
   const bool is_v = warp & 1;
   const int64_t sp = is_v ? p.v_sp : p.k_sp, ss = is_v ? p.v_ss : p.k_ss, sh = is_v ? p.v_sh : p.k_sh;
-  const uint16_t* src = (is_v ? p.v_src : p.k_src) + page_from * sp + row_from * ss;
-  uint16_t* dst = (is_v ? p.v_dst : p.k_dst) + page_to * sp + row_to * ss;
-  for (int h = 0; h < p.heads_kv; h += kCopyUnroll) {
-    uint4 x[kCopyUnroll][2];
+  // lanes 0 .. 3: one head row each
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * (kCopyWarps / 2) + (warp >> 1)) * kCopyRows + lane;
+  const int place = static_cast<int>(min(row / p.heads_kv, static_cast<int64_t>(p.keep)));
+  const int h = static_cast<int>(row % p.heads_kv);
+  int64_t from = 0, to = 0;
+  bool moves = false;
+  pdl_wait();
+  if (lane < kCopyRows && place < p.keep) {
+    const int64_t at = static_cast<int64_t>(b) * p.keep + place;
+    const int slot = p.kept[at];
+    if (h == 0 && !is_v) p.new_weights[at] = slot < 0 ? 0.f : __ldg(p.weights + b * p.weights_stride + slot);
+    if (slot >= 0) {
+      int entry, in_page;
+      split_slot(p.from, slot, entry, in_page);
+      const int page_from = page_of(p.from, b, entry);
+      from = page_from * sp + in_page * ss + h * sh;
+      split_slot(p.to, place, entry, in_page);
+      const int page_to = page_of(p.to, b, entry);
+      to = page_to * sp + in_page * ss + h * sh;
+      moves = page_ok(p.from, page_from) && page_ok(p.to, page_to);
+      if (!moves && p.status) atomicCAS(p.status, 0, ST_BAD_PAGE);
+    }
+  }
+  const unsigned rows = __ballot_sync(0xffffffffu, moves);
+  uint4 x[kCopyRows][2];
 #pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u)
-      if (h + u < p.heads_kv) {
-        const uint4* s = reinterpret_cast<const uint4*>(src + (h + u) * sh);
-        x[u][0] = __ldcs(s + lane), x[u][1] = __ldcs(s + lane + 32);
-      }
+  for (int u = 0; u < kCopyRows; ++u) {
+    const int64_t at = __shfl_sync(0xffffffffu, from, u);
+    if (rows >> u & 1) {
+      const uint4* s = reinterpret_cast<const uint4*>((is_v ? p.v_src : p.k_src) + at);
+      x[u][0] = __ldcs(s + lane), x[u][1] = __ldcs(s + lane + 32);
+    }
+  }
 #pragma unroll
-    for (int u = 0; u < kCopyUnroll; ++u)
-      if (h + u < p.heads_kv) {
-        uint4* d = reinterpret_cast<uint4*>(dst + (h + u) * sh);
-        __stcs(d + lane, x[u][0]);
-        __stcs(d + lane + 32, x[u][1]);
-      }
+  for (int u = 0; u < kCopyRows; ++u) {
+    const int64_t at = __shfl_sync(0xffffffffu, to, u);
+    if (rows >> u & 1) {
+      uint4* d = reinterpret_cast<uint4*>((is_v ? p.v_dst : p.k_dst) + at);
+      __stcs(d + lane, x[u][0]);
+      __stcs(d + lane + 32, x[u][1]);
+    }
   }
 }
 
@@ -314,6 +324,9 @@ int launch_evict(const splitd_evict_params* a, cudaStream_t stream) {
   const int64_t share = one ? slots : (slots + ev::kCluster - 1) / ev::kCluster;
   p.cached = static_cast<int>(share < ev::kCacheMost ? share : ev::kCacheMost);
   if (int e = allow_cache(one ? ev::splitd_evict_select_kernel<1> : ev::splitd_evict_select_kernel<ev::kCluster>, one)) return e;
+  constexpr int kBlockRows = ev::kCopyRows * ev::kCopyWarps / 2;
+  const int64_t copy_blocks = (static_cast<int64_t>(a->keep) * a->heads_kv + kBlockRows - 1) / kBlockRows;
+  if (copy_blocks > 0x7fffffff) return fail(SPLITD_ERR_INVALID_ARGUMENT, "eviction: keep * heads_kv is too large");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(one ? a->batch : a->batch * ev::kCluster);
   cfg.blockDim = dim3(ev::kThreads);
@@ -328,7 +341,7 @@ int launch_evict(const splitd_evict_params* a, cudaStream_t stream) {
                        : cudaLaunchKernelEx(&cfg, ev::splitd_evict_select_kernel<ev::kCluster>, p);
   if (ce == cudaSuccess)
     ce = launch_dependent(ev::splitd_evict_copy_kernel,
-                          dim3((a->keep + ev::kCopyWarps / 2 - 1) / (ev::kCopyWarps / 2), a->batch),
+                          dim3(static_cast<unsigned>(copy_blocks), a->batch),
                           dim3(ev::kCopyWarps * 32), 0, stream, p);
   if (ce != cudaSuccess) {
     cudaGetLastError();

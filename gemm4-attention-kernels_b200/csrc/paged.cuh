@@ -23,7 +23,7 @@ struct PageMap {
 // Slots that the table can address.
 __host__ __device__ inline int page_capacity(const PageMap& m) {
   const int64_t n = static_cast<int64_t>(m.max_pages) * m.page_size;
-  constexpr int64_t kMost = 0x7fffffff - 4096;  // slots plus a tile stay below 2^31
+  constexpr int64_t kMost = 0x7fffffff - 65536;  // a slot plus a step of any loop over slots stays below 2^31
   return static_cast<int>(n < kMost ? n : kMost);
 }
 __host__ inline int page_shift(int page_size) {

@@ -929,7 +929,8 @@ int launch_paged_attn(const splitd_paged_params* a, cudaStream_t stream) {
   cudaError_t ce = cudaGetLastError();
   // Few rows (so few units, each shared by many CTAs): four blocks a row, in which sixteen groups of threads read partial
   // results side by side (1 x 131072 keys, 32 rows, 37 results each: 4 us, 7 us with one block of four groups a row). More
-  // rows: one small block each (8 x 230 keys, 512 rows, 8 results each: ... us, 19 us the other way). The choice, which
+  // rows: one small block each (8 x 230 keys, 512 rows, 8 results each: 12 us in
+  // all, 26 us the other way). The choice, which
   // decides the order of the sums, does not look at the width of the page table.
   const bool few = static_cast<int64_t>(p.batch) * p.heads_kv * p.rows <= sm_count();
   const int64_t longest = !p.weights ? 0 : max_keys(a) < p.weights_len ? max_keys(a) : p.weights_len;

@@ -137,6 +137,7 @@ int splitd_paged_evict(const splitd_evict_params* p, void* stream) {
     return fail(SPLITD_ERR_INVALID_ARGUMENT, "a tensor is NULL");
   if (int e = check_heads(p->heads_kv, p->heads_kv, p->head_dim, SPLITD_DTYPE_BF16)) return e;
   if (int e = check_pages(p->batch, p->num_pages, p->page_size, p->max_pages)) return e;
+  if (p->keep > 1 << 30) return fail(SPLITD_ERR_INVALID_ARGUMENT, "keep must be at most 2^30, got %d", p->keep);
   if (p->keep <= 0 || p->keep_first < 0 || p->keep_recent < 0 ||
       static_cast<int64_t>(p->keep_first) + p->keep_recent > p->keep)
     return fail(SPLITD_ERR_INVALID_ARGUMENT, "keep must be > 0 and at least keep_first + keep_recent, got %d, %d, %d", p->keep,

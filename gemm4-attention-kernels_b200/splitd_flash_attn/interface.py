@@ -300,7 +300,8 @@ def _status_flag(device: torch.device) -> torch.Tensor:
     key = device.index if device.index is not None else torch.cuda.current_device()
     flag = _status_flags.get(key)
     if flag is None:
-        flag = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # it outlives the mode that the first call happens to run in
+            flag = torch.zeros(1, dtype=torch.int32, device=device)
         _status_flags[key] = flag
     return flag
 

@@ -81,6 +81,12 @@ def _check_cache(k_pages, v_pages, page_table, seqlens_k, page_table_name="page_
     _check_table(page_table, page_table_name, seqlens_k.shape[0], device)
 
 
+def _check_written(k_pages, v_pages) -> None:
+    for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+            raise ValueError(f"{name} is written and must not be an expanded tensor, got strides {t.stride()}")
+
+
 def _check_table(page_table, name, batch, device) -> None:
     if page_table.ndim != 2 or page_table.shape[0] != batch:
         raise ValueError(f"{name} has shape {tuple(page_table.shape)}, expected ({batch}, pages per sequence)")
@@ -113,6 +119,8 @@ def _check_weights(key_weights, batch, device) -> None:
     _check_same(key_weights, "key_weights", torch.float32, device)
     if key_weights.shape[1] > 1 and key_weights.stride(1) != 1:
         raise ValueError("key_weights must have an innermost stride of 1")
+    if batch > 1 and key_weights.stride(0) < key_weights.shape[1]:
+        raise ValueError("the rows of key_weights must not overlap")
 
 
 def _unit_rows(*tensors) -> bool:
@@ -281,6 +289,7 @@ def _check_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, po
     _check_heads(k, "k", rank)
     _check_heads(v, "v", rank)
     _check_cache(k_pages, v_pages, page_table, seqlens_k)
+    _check_written(k_pages, v_pages)
     if v.shape != k.shape:
         raise ValueError(f"v has shape {tuple(v.shape)}, expected {tuple(k.shape)}")
     if k.shape[-2] != k_pages.shape[2]:
@@ -364,6 +373,8 @@ def _paged_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, po
     p = _capi.SplitdAppendParams.from_buffer_copy(plan.params)
     p.k, p.v = k_at, v_at
     p.k_pages, p.v_pages = _page_pointers(k_pages, v_pages)
+    if p.k_pages == p.v_pages and k_pages.numel():
+        raise ValueError("k_pages and v_pages must not be the same memory: both are written")
     p.page_table, p.seqlens_k = page_table.data_ptr() or _NO_MEMORY, seqlens_k.data_ptr() or _NO_MEMORY
     if q is not None:
         p.q, p.q_out = q_at, q_out.data_ptr()
@@ -456,18 +467,19 @@ def split_paged_append_func(
 
 def _check_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent) -> None:
     _check_cache(k_pages, v_pages, page_table, seqlens_k)
+    _check_written(k_pages, v_pages)
     batch = seqlens_k.shape[0]
     _check_weights(key_weights, batch, k_pages.device)
     _check_table(new_page_table, "new_page_table", batch, k_pages.device)
     for name, n in (("keep", keep), ("keep_first", keep_first), ("keep_recent", keep_recent)):
-        if isinstance(n, bool) or not isinstance(n, int):
+        if isinstance(n, bool) or not isinstance(n, (int, torch.SymInt)):
             raise TypeError(f"{name} must be an int, got {type(n).__name__}")
         if n < 0:
             raise ValueError(f"{name} must be non-negative, got {n}")
     if keep < 1 or keep < keep_first + keep_recent:
         raise ValueError(f"keep ({keep}) must be at least 1 and at least keep_first + keep_recent ({keep_first} + {keep_recent})")
-    if keep > 2**31 - 1:
-        raise ValueError(f"keep ({keep}) does not fit 32 bits")
+    if keep > 2**30:
+        raise ValueError(f"keep ({keep}) must be at most 2^30")
     if new_page_table.shape[1] * k_pages.shape[1] < keep:
         raise ValueError(
             f"new_page_table has {new_page_table.shape[1]} pages of {k_pages.shape[1]} slots per sequence, too few for {keep}"

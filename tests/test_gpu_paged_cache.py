@@ -148,6 +148,66 @@ def test_append_strided_tokens_and_caches():
     assert torch.equal(a, b) and torch.equal(kv[:, 0], k_pages) and torch.equal(kv[:, 1], v_pages)
 
 
+def test_append_refuses_one_memory_for_keys_and_values_and_misaligned_caches():
+    from splitd_flash_attn import split_flash_attn_paged_func, split_paged_append_func
+
+    k_pages, v_pages, table, seqlens, _ = make_cache([20], 16, 2, torch.bfloat16, 1, fill=7.0)
+    k = tokens((1, 1), 2, torch.bfloat16, 2)
+    with pytest.raises(ValueError, match="same memory"):
+        split_paged_append_func(None, k, k, k_pages, k_pages, table, seqlens)
+    odd = torch.zeros(k_pages.numel() + 4, dtype=torch.bfloat16, device="cuda")[4:].view(k_pages.shape)
+    with pytest.raises(ValueError, match="16-byte"):
+        split_paged_append_func(None, k, k, odd, v_pages, table, seqlens)
+    with pytest.raises(ValueError, match="16-byte"):
+        split_flash_attn_paged_func(k, k_pages, odd, table, seqlens)
+    # reading keys and values from one memory is fine, as in the dense attention
+    a = split_flash_attn_paged_func(k, k_pages, k_pages, table, seqlens)
+    assert torch.equal(a, split_flash_attn_paged_func(k, k_pages, k_pages.clone(), table, seqlens))
+
+
+def test_misaligned_contiguous_tokens_are_copied():
+    from splitd_flash_attn import split_flash_attn_paged_func, split_paged_append_func, split_rotary_func
+
+    k_pages, v_pages, table, seqlens, _ = make_cache([20, 5], 16, 2, torch.bfloat16, 1, fill=7.0)
+    q, k = tokens((2, 1), 8, torch.bfloat16, 2), tokens((2, 1), 2, torch.bfloat16, 3)
+
+    def shifted(t):
+        s = torch.zeros(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape)
+        s.copy_(t)
+        assert s.is_contiguous() and s.data_ptr() % 16
+        return s
+
+    caches = [(k_pages.clone(), v_pages.clone()) for _ in range(2)]
+    a = split_paged_append_func(q, k, k, *caches[0], table, seqlens, inv_freq=freq(512))
+    b = split_paged_append_func(shifted(q), shifted(k), shifted(k), *caches[1], table, seqlens, inv_freq=freq(512))
+    assert torch.equal(a, b) and all(torch.equal(x, y) for x, y in zip(*caches))
+    assert torch.equal(split_flash_attn_paged_func(q, *caches[0], table, seqlens), split_flash_attn_paged_func(shifted(q), *caches[0], table, seqlens))
+    pos = torch.arange(1, device="cuda")
+    assert torch.equal(split_rotary_func(q, k, pos, freq(512))[1], split_rotary_func(q, shifted(k), pos, freq(512))[1])
+
+
+def test_under_inference_mode_and_after_it():
+    from splitd_flash_attn import split_flash_attn_paged_func, split_paged_append_func
+    from splitd_flash_attn import interface
+    from splitd_flash_attn.interface import kernel_status, reset_kernel_status
+
+    k_pages, v_pages, table, seqlens, _ = make_cache([21, 5], 16, 1, torch.bfloat16, 1, fill=7.0)
+    q, k = tokens((2, 1), 5, torch.bfloat16, 2), tokens((2, 1), 1, torch.bfloat16, 3)
+    saved = interface._status_flags.copy()
+    interface._status_flags.clear()
+    try:
+        with torch.inference_mode():
+            qr = split_paged_append_func(q, k, k, k_pages, v_pages, table, seqlens, inv_freq=freq(512))
+            a = split_flash_attn_paged_func(qr, k_pages, v_pages, table, seqlens)
+        qr = split_paged_append_func(q, k, k, k_pages, v_pages, table, seqlens, inv_freq=freq(512))
+        b = split_flash_attn_paged_func(qr, k_pages, v_pages, table, seqlens)
+        assert torch.equal(a, b) and not b.is_inference()
+        reset_kernel_status()
+        assert kernel_status() == 0
+    finally:
+        interface._status_flags.update(saved)
+
+
 # ---------------------------------------------------------------------------
 # eviction
 # ---------------------------------------------------------------------------

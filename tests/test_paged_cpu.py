@@ -145,7 +145,7 @@ def test_evict_entry_point_refuses():
         return p
 
     for field, value, text in (
-        ("kept", None, "NULL"), ("keep", 0, "keep"), ("keep", 33, "do not hold"), ("keep_first", -1, "keep"), ("keep_recent", 33, "keep"),
+        ("kept", None, "NULL"), ("keep", 0, "keep"), ("keep", (1 << 30) + 1, "2^30"), ("keep", 33, "do not hold"), ("keep_first", -1, "keep"), ("keep_recent", 33, "keep"),
         ("new_max_pages", -1, "do not hold"), ("key_weights_len", -1, "key_weights_len"), ("batch", 70000, "batch"),
         ("k_strides", (1, 8, 8), "multiple of 8"),
     ):
@@ -218,6 +218,8 @@ def test_attention_function_checks(fake):
         fn(q, k, v, t, n, key_weights=w.double())
     with pytest.raises(ValueError, match="key_weights"):
         fn(q, k, v, t, n, key_weights=torch.empty(64, 3, device="cuda").T)
+    with pytest.raises(ValueError, match="overlap"):
+        fn(q, k, v, t, n, key_weights=w[:1].expand(3, -1))
     with pytest.raises(TypeError, match="tuple"):
         fn(q, k, v, t, n, window_size=[1, 2])
     with pytest.raises(NotImplementedError, match="backward"):
@@ -264,6 +266,8 @@ def test_append_function_checks(fake):
         fn(q, k, k, k_pages, v_pages, t, n, inv_freq=f, positions=pos[:2])
     with pytest.raises(TypeError, match="k_pages"):
         fn(q, k, k, k_pages.half(), v_pages.half(), t, n)
+    with pytest.raises(ValueError, match="expanded"):
+        fn(q, k, k, k_pages, v_pages[:1].expand(10, -1, -1, -1), t, n)
     with pytest.raises(NotImplementedError, match="backward"):
         fn(q, k.requires_grad_(), k, k_pages, v_pages, t, n)
 
@@ -289,6 +293,10 @@ def test_evict_function_checks(fake):
         fn(k, v, t, n, w, new.long(), 4)
     with pytest.raises(ValueError, match="key_weights"):
         fn(k, v, t, n, w[0], new, 4)
+    with pytest.raises(ValueError, match="2\^30"):
+        fn(k, v, t, n, w, new, 2**30 + 1)
+    with pytest.raises(ValueError, match="expanded"):
+        fn(k[:1].expand(10, -1, -1, -1), v, t, n, w, new, 4)
 
 
 def test_rotary_function_checks(fake):
