@@ -7,13 +7,12 @@
 // lse = (m + log2 l) ln 2; a row that sees no key has l = 0: o = 0, lse = -inf.
 //
 // What bounds it. Every visible key costs 2 KB of cache and 4 * 512 * R flops: at R = 8, 8 flops a byte, far left of the
-// ridge. So the kernel is built around the stream of cache rows: one CTA per SM, four producer warps that keep a ring of
-// 32-row stages full with one 1 KB bulk copy per row (a page of any size and a row of any page are then the same thing:
-// no tile has to match a page), and eight warps that compute. One producer warp alone can issue such a copy every 74
-// cycles, 59 % of the bandwidth. Measured: 1 x 131072 keys, 4 KV heads, 8 rows each: 158 us, 6.8 TB/s; 32 sequences of up
-// to 8192: 206 us, 6.8 TB/s (a plain copy moves 6.6). With 32 rows (4 tokens) a tile's instructions are what bounds it:
-// two computing warps per scheduler wait out their fixed latencies (tensor pipe 42 %, issue slots 40 %), 119 us where
-// the stream alone takes 94.
+// ridge. So the kernel is built around the stream of cache rows: one CTA per SM, four producer warps that keep two rings
+// of 32-row stages (keys, values) full with one 1 KB bulk copy per row (a page of any size and a row of any page are then
+// the same thing: no tile has to match a page). One producer warp alone can issue such a copy every 74 cycles, 59 % of
+// the bandwidth. Measured: 1 x 131072 keys, 4 KV heads, 8 rows each: 158 us, 6.8 TB/s; 32 sequences of up to 8192: 207 us,
+// 6.7 TB/s (a plain copy moves 6.6). With 32 rows (4 tokens) a tile's instructions cost as much as its bytes: 103 us
+// where the stream alone takes 94 and the bytes 81.
 //
 // Split. The (sequence, KV head, row block) units are laid end to end, in tiles of 32 keys, and every CTA takes an
 // equal share of the whole line, whatever the lengths are; the lengths never leave the device. A unit that lies inside
@@ -21,11 +20,13 @@
 // the workspace in fp32, and a second kernel adds them up in CTA order: no atomics, the same bits every time.
 //
 // Products. keys x rows on the warp matrix instruction (16 keys x 8 rows x 16): the cache row is the A operand, so a
-// group of 8 query heads fills the 8 columns exactly. S^T = K Q^T is split over two key halves and four quarters of
-// the head dimension; the four partial sums meet in shared memory, where warp w then owns the softmax of rows w,
-// w + 8, ... with one key per lane. O^T = V^T P^T is split over the head dimension, 64 columns per warp, accumulators
-// in registers. P is kept as the sum of TWO 16-bit numbers (two products): a single one would put an error of the size
-// of the output's own rounding on top of it.
+// group of 8 query heads fills the 8 columns exactly. S^T = K Q^T is split over four quarters of the head dimension; the
+// partial sums meet in shared memory, where score warp w then owns the softmax of every fourth (eighth) row, one key per
+// lane. O^T = V^T P^T is split over the head dimension, 64 columns per value warp, accumulators in registers. Score and
+// value warps only meet through two buffers of P, so that products and softmax of neighbouring tiles overlap (one set of
+// eight warps for both, with one barrier a tile: 119 us with 32 rows, 103 us this way; up to 24 rows the same). P is kept
+// as the sum of TWO 16-bit numbers (two products): a single one would put an error of the size of the output's own
+// rounding on top of it.
 #include <cstring>
 
 #include "launch.cuh"
@@ -38,21 +39,36 @@ namespace pa {
 constexpr int kTile = 32;                      // keys per tile = rows per ring stage
 constexpr int kPitch = kRowBytes + 16;         // ldmatrix reads 8 rows at once: 16 bytes of padding spread them over the banks
 constexpr int kStageBytes = kTile * kPitch;
-constexpr int kWarps = 8;                      // warps that compute
 constexpr int kProducers = 4;                  // producer warps: each asks for a quarter of a tile's rows
 constexpr int kRowsPerProducer = kTile / kProducers;
-constexpr int kThreads = 32 * (kWarps + kProducers);
+constexpr int kValueWarps = 8;                 // 64 columns of the head dimension each
+// Score warps have a quarter of the head dimension each; from 25 rows on half of the rows, too (32 rows: 103 us, 115 us
+// with four score warps; they read the keys from shared memory twice then, which 24 rows would not repay).
+template <int kNB>
+constexpr int kRowGroups = kNB == 4 ? 2 : 1;
+template <int kNB>
+constexpr int kScoreWarps = 4 * kRowGroups<kNB>;
+template <int kNB>
+constexpr int kThreads = 32 * (kValueWarps + kScoreWarps<kNB> + kProducers);
 constexpr int kPartPitch = 36;                 // floats per row of the partial scores (32 keys + padding)
 constexpr int kPPitch = 20;                    // 32-bit words per row of P (32 keys x 2 bytes + padding)
 constexpr int kMaxRows = 32;                   // rows of a row block
 
-// From 17 rows on a computing thread needs more than the 168 registers that 384 threads can have each, so the producers
-// give up some of theirs (4 tokens, 32 rows: 305 us with spills, 159 us with the split; with 8 rows the split costs 1 %).
-// The launch checks that the block comes with at least as many as the two shares together. Sixteen computing warps were
-// tried instead: no faster with 16 rows, and 155 against 119 us with 32, where they read every row twice.
+// From 17 rows on some warps need more registers than a block's threads can have each (512: 128, 640: 96), and the others
+// give up some of theirs. The launch checks that the block comes with at least as many as the shares together.
 template <int kNB>
 constexpr bool kSplitRegs = kNB >= 3;
-constexpr int kProducerRegs = 56, kConsumerRegs = 216;
+template <int kNB>
+constexpr int kProducerRegs = kNB == 4 ? 40 : 48;
+template <int kNB>
+constexpr int kScoreRegs = kNB == 4 ? 104 : 168;
+template <int kNB>
+constexpr int kValueRegs = kNB == 4 ? 112 : 120;
+template <int kNB>
+constexpr int kSplitTotal =
+    32 * (kProducers * kProducerRegs<kNB> + kScoreWarps<kNB> * kScoreRegs<kNB> + kValueWarps * kValueRegs<kNB>);
+static_assert(kSplitTotal<3> <= 65536 / kThreads<3> / 8 * 8 * kThreads<3> && kSplitTotal<4> <= 65536 / kThreads<4> / 8 * 8 * kThreads<4>,
+              "registers of a block");
 
 struct Desc {  // what the producer tells the others about a stretch of tiles
   int b, head, row0, n_tiles;  // n_tiles == 0: no more work
@@ -67,10 +83,11 @@ struct Layout {
   // two of each of these: one tile's are read while the next one's are written
   static constexpr int kPartFloats = 4 * kRows * kPartPitch;
   static constexpr int kPWords = kRows * kPPitch;  // of each half of P
-  // Enough stages in flight to cover the latency of HBM, and no more: six would fit beside 8 rows, but the deeper queue of
-  // requests costs HBM efficiency (1 x 131072 keys: 172 us with six, 168 with five, 159 with four, 160 with three;
-  // 32 sequences up to 8192: 222, 215, 208, 210). With 32 rows a stage is held longer (119 us with five, 125 with four).
-  static constexpr int kStages = kNB <= 2 ? 4 : 5;
+  // Of keys (and query rows), and of values: enough to cover the latency of HBM, and no more, since a deeper queue of
+  // requests costs HBM efficiency (1 x 131072 keys: 172 us with six stages in all, 168 with five, 159 with four, 160 with
+  // three; 32 sequences up to 8192: 222, 215, 208, 210).
+  static constexpr int kKStages = 2, kVStages = 2;
+  static constexpr int kStages = kKStages + kVStages;
   static constexpr int kOffPart = kStages * kStageBytes;
   static constexpr int kOffP = kOffPart + 2 * kPartFloats * 4;
   static constexpr int kOffCorr = kOffP + 2 * 2 * kPWords * 4;
@@ -78,7 +95,8 @@ struct Layout {
   static constexpr int kOffBounds = kOffStat + kRows * 8;
   static constexpr int kOffDesc = kOffBounds + kRows * 8;
   static constexpr int kOffBar = kOffDesc + kStages * static_cast<int>(sizeof(Desc));
-  static constexpr int kOffAbort = kOffBar + 2 * kStages * 8;
+  static constexpr int kBars = 2 * kStages + 6;
+  static constexpr int kOffAbort = kOffBar + kBars * 8;
   static constexpr int kBytes = kOffAbort + 16;
   static_assert(kOffDesc % 16 == 0 && kOffBar % 8 == 0 && kOffPart % 16 == 0, "alignment");
   static_assert(kBytes <= 232448, "shared memory of an SM");
@@ -175,28 +193,67 @@ __device__ __forceinline__ float warp_max(float x) {
   return y;
 }
 
+// A ring of kStages slots: 32-row stages (of keys or of values), buffers of P, or the one place for a unit's (m, l).
 template <int kStages>
 struct Ring {
   uint32_t full, empty;  // barrier arrays
   int stage = 0;
   uint32_t phase = 0;
+  __device__ __forceinline__ Ring(uint32_t bars) : full(bars), empty(bars + 8 * kStages) {}
   __device__ __forceinline__ void next() {
     if (++stage == kStages) stage = 0, phase ^= 1;
+  }
+  __device__ __forceinline__ bool wait_full(volatile int* abort_flag, int* status, int code) const {
+    return mbar_wait(full + 8 * stage, phase, abort_flag, status, code);
+  }
+  __device__ __forceinline__ bool wait_empty(volatile int* abort_flag, int* status, int code) const {
+    return mbar_wait(empty + 8 * stage, phase ^ 1, abort_flag, status, code);
+  }
+  // one arrival per warp
+  __device__ __forceinline__ void arrive_full(int lane) const {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(full + 8 * stage);
+  }
+  __device__ __forceinline__ void arrive_empty(int lane) const {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + 8 * stage);
+  }
+};
+template <int kNB>
+struct Rings {
+  using L = Layout<kNB>;
+  Ring<L::kKStages> k;
+  Ring<L::kVStages> v;
+  Ring<2> p;
+  Ring<1> stat;
+  __device__ __forceinline__ explicit Rings(uint32_t bars)
+      : k(bars), v(bars + 16 * L::kKStages), p(bars + 16 * L::kStages), stat(bars + 16 * L::kStages + 32) {}
+  __device__ __forceinline__ void init() const {
+    auto one = [](const auto& r, int n, int full, int empty) {
+      for (int i = 0; i < n; ++i) mbar_init(r.full + 8 * i, full), mbar_init(r.empty + 8 * i, empty);
+    };
+    one(k, L::kKStages, kProducers, kScoreWarps<kNB>);
+    one(v, L::kVStages, kProducers, kValueWarps);
+    one(p, 2, kScoreWarps<kNB>, kValueWarps);
+    one(stat, 1, kScoreWarps<kNB>, kValueWarps);
   }
 };
 
 template <int kNB>
-__device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem, Ring<Layout<kNB>::kStages> r, volatile int* abort_flag, int pw,
+__device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem, Rings<kNB> rings, volatile int* abort_flag, int pw,
                                          int lane) {
   using L = Layout<kNB>;
   const int my_row = pw * kRowsPerProducer + lane % kRowsPerProducer;  // row of a tile; lanes beyond kRowsPerProducer are idle
   const bool active = lane < kRowsPerProducer;
   Desc* descs = reinterpret_cast<Desc*>(smem + L::kOffDesc);
-  const uint32_t ring0 = smem_u32(smem);
-  int used = 0;  // stages handed out
+  auto& kr = rings.k;
+  auto& vr = rings.v;
+  const uint32_t k_ring = smem_u32(smem), v_ring = k_ring + L::kKStages * kStageBytes;
+  Desc* const v_descs = descs + L::kKStages;
+  int k_used = 0, v_used = 0;  // stages handed out
   bool ok = true;
-  auto acquire = [&]() {
-    if (ok) ok = mbar_wait(r.empty + 8 * r.stage, r.phase ^ 1, abort_flag, p.status, ST_TIMEOUT_LOAD);
+  auto acquire = [&](const auto& r) {
+    if (ok) ok = r.wait_empty(abort_flag, p.status, ST_TIMEOUT_LOAD);
     ok = __all_sync(0xffffffffu, ok);
     return ok;
   };
@@ -246,20 +303,19 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
       const int n_rows = min(p.rows_per_block, p.rows - row0);
       const int lo = first_key(p, len);
       // query rows: one ring stage, with the description of the work in front of it
-      if (!acquire()) break;
+      if (!acquire(kr)) break;
+      Desc d;
+      d.b = b, d.head = head, d.row0 = row0, d.n_tiles = n;
+      d.len = len, d.first_key = lo + tile0 * kTile;
+      d.slot = n == n_tiles ? -1 : (tile0 > 0 ? 0 : 1);
+      d.pad = 0;
       {
-        const uint32_t bar = r.full + 8 * r.stage;
+        const uint32_t bar = kr.full + 8 * kr.stage;
+        const uint32_t dst = k_ring + kr.stage * kStageBytes + my_row * kPitch;
         const uint32_t rows = __popc(__ballot_sync(0xffffffffu, active && my_row < n_rows));
-        if (lane == 0 && pw == 0) {
-          Desc d;
-          d.b = b, d.head = head, d.row0 = row0, d.n_tiles = n;
-          d.len = len, d.first_key = lo + tile0 * kTile;
-          d.slot = n == n_tiles ? -1 : (tile0 > 0 ? 0 : 1);
-          d.pad = 0;
-          descs[r.stage] = d;
-        }
+        if (lane == 0 && pw == 0) descs[kr.stage] = d;
         if (active && my_row >= n_rows && my_row < L::kRows) {  // rows that pad the block: scores of 0, and no NaN
-          for (int c = 0; c < kRowBytes; c += 16) st_shared_v4(ring0 + r.stage * kStageBytes + my_row * kPitch + c, 0, 0, 0, 0);
+          for (int c = 0; c < kRowBytes; c += 16) st_shared_v4(dst + c, 0, 0, 0, 0);
           fence_proxy_async_smem();
         }
         __syncwarp();
@@ -267,10 +323,9 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
         __syncwarp();
         if (active && my_row < n_rows) {
           const int i = (row0 + my_row) / p.group, g = (row0 + my_row) - i * p.group;
-          bulk_load(ring0 + r.stage * kStageBytes + my_row * kPitch, p.q + b * p.q_sb + i * p.q_ss + (head * p.group + g) * p.q_sh,
-                    kRowBytes, bar);
+          bulk_load(dst, p.q + b * p.q_sb + i * p.q_ss + (head * p.group + g) * p.q_sh, kRowBytes, bar);
         }
-        r.next(), ++used;
+        kr.next(), ++k_used;
       }
       // keys and values: lane = row of the tile; the page of the next tile is looked up one tile ahead
       auto lookup = [&](int slot, int& page, int& row) {
@@ -285,10 +340,9 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
       lookup(slot, page, row);
       const uint16_t* v_src = nullptr;
       bool v_have = false;
-      auto ask = [&](const uint16_t* src, bool have) {
-        if (!acquire()) return;
+      auto ask = [&](auto& r, uint32_t ring, int& used, const uint16_t* src, bool have) {
         const uint32_t bar = r.full + 8 * r.stage;
-        const uint32_t dst = ring0 + r.stage * kStageBytes + my_row * kPitch;
+        const uint32_t dst = ring + r.stage * kStageBytes + my_row * kPitch;
         if (active && !have) {  // a row that is not there counts as zeros: 0 * (what lay there) could be NaN
           for (int c = 0; c < kRowBytes; c += 16) st_shared_v4(dst + c, 0, 0, 0, 0);
           fence_proxy_async_smem();
@@ -299,15 +353,18 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
         if (have) bulk_load(dst, src, kRowBytes, bar);
         r.next(), ++used;
       };
-      // in the order of use: K(0), K(1), V(0), K(2), V(1), ..., K(n - 1), V(n - 2), V(n - 1)
+      // K(0), K(1), V(0), K(2), V(1), ..., K(n - 1), V(n - 2), V(n - 1)
       for (int i = 0; i <= n && ok; ++i) {
         int next_page = -1, next_row = 0;
         if (i + 1 < n) lookup(slot + kTile, next_page, next_row);
         const bool inside = active && i < n && slot < len;
         const bool have = inside && page_ok(p.map, page);
         if (inside && !have && p.status) atomicCAS(p.status, 0, ST_BAD_PAGE);
-        if (i < n) ask(p.k + page * p.k_sp + row * p.k_ss + head * p.k_sh, have);
-        if (i > 0) ask(v_src, v_have);
+        if (i < n && acquire(kr)) ask(kr, k_ring, k_used, p.k + page * p.k_sp + row * p.k_ss + head * p.k_sh, have);
+        if (i > 0 && acquire(vr)) {
+          if (i == 1 && lane == 0 && pw == 0) v_descs[vr.stage] = d;
+          ask(vr, v_ring, v_used, v_src, v_have);
+        }
         v_src = p.v + page * p.v_sp + row * p.v_ss + head * p.v_sh, v_have = have;
         slot += kTile, page = next_page, row = next_row;
       }
@@ -323,87 +380,81 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
       }
     }
   }
-  if (acquire()) {
+  // no more work, on both rings
+  auto finish = [&](auto& r, Desc* at) {
     if (lane == 0) {
-      if (pw == 0) descs[r.stage].n_tiles = 0;
+      if (pw == 0) at[r.stage].n_tiles = 0;
       mbar_arrive(r.full + 8 * r.stage);
     }
-  } else {
-    // a wait was given up: let the copies in flight land before the block ends
-    for (int i = 0; i < L::kStages && i < used; ++i) {
-      r.phase ^= r.stage == 0;
-      r.stage = r.stage == 0 ? L::kStages - 1 : r.stage - 1;
-      volatile int never = 0;
-      mbar_wait_limit(r.full + 8 * r.stage, r.phase, &never, nullptr, 0, 1000ull * 1000ull * 1000ull);
-    }
+  };
+  if (acquire(kr)) finish(kr, descs);
+  if (acquire(vr)) finish(vr, v_descs);
+  if (!ok) {  // a wait was given up: let the copies in flight land before the block ends
+    auto drain = [&](auto& r, int stages, int used) {
+      for (int i = 0; i < stages && i < used; ++i) {
+        r.phase ^= r.stage == 0;
+        r.stage = r.stage == 0 ? stages - 1 : r.stage - 1;
+        volatile int never = 0;
+        mbar_wait_limit(r.full + 8 * r.stage, r.phase, &never, nullptr, 0, 1000ull * 1000ull * 1000ull);
+      }
+    };
+    drain(kr, L::kKStages, k_used);
+    drain(vr, L::kVStages, v_used);
   }
 }
 
+// Four or eight warps: S^T = K Q^T, a quarter of the head dimension (and half of the rows) each, and the softmax of every
+// fourth or eighth row.
 template <bool kFp16, int kNB>
-__device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem, Ring<Layout<kNB>::kStages> r,
-                                         volatile int* abort_flag, int warp, int lane) {
+__device__ __forceinline__ void score_warp(const PagedAttnParams& p, uint8_t* smem, Rings<kNB> rings, volatile int* abort_flag,
+                                           int warp, int lane) {
   using L = Layout<kNB>;
   constexpr int kRows = L::kRows;
-  constexpr int kMT = kHeadDim / kWarps / 16;  // values: 16-column tiles of a warp
-  constexpr int kR = kRows / kWarps;           // softmax: rows of a warp (w, w + kWarps, ...)
-  static_assert(kWarps == 2 * 4, "scores: two key halves times four quarters of the head dimension");
+  constexpr int kW = kScoreWarps<kNB>;
+  constexpr int kNBS = kNB / kRowGroups<kNB>;  // n tiles of a warp
+  constexpr int kR = kRows / kW;               // softmax: rows of a warp
+  const int quarter = warp & 3, nb0 = (warp >> 2) * kNBS;
   const Desc* descs = reinterpret_cast<const Desc*>(smem + L::kOffDesc);
   float* part0 = reinterpret_cast<float*>(smem + L::kOffPart);
-  uint32_t* p0 = reinterpret_cast<uint32_t*>(smem + L::kOffP);
+  uint16_t* p0 = reinterpret_cast<uint16_t*>(smem + L::kOffP);
   float* corr0 = reinterpret_cast<float*>(smem + L::kOffCorr);
   float2* stat = reinterpret_cast<float2*>(smem + L::kOffStat);
   int2* bounds = reinterpret_cast<int2*>(smem + L::kOffBounds);
+  auto& r = rings.k;
   const uint32_t ring0 = smem_u32(smem);
-  const int key_half = warp & 1, d_quarter = warp >> 1;
   const int frag_row = lane >> 2, frag_col = (lane & 3) * 2;
   const float scale_log2 = p.scale * kLog2e;
   const float cap_in = p.softcap > 0.f ? p.scale / p.softcap : 0.f;
   const float cap_out = p.softcap * kLog2e;
-
-  auto wait_full = [&]() { return mbar_wait(r.full + 8 * r.stage, r.phase, abort_flag, p.status, ST_TIMEOUT_SOFTMAX); };
-  auto release = [&]() {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(r.empty + 8 * r.stage);
-    r.next();
-  };
-  auto sync = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kWarps) : "memory"); };
+  auto wait = [&](const auto& ring) { return ring.wait_full(abort_flag, p.status, ST_TIMEOUT_SOFTMAX); };
 
   while (true) {
-    bool ok = wait_full();
-    // All of these warps have to agree on whether to go on, or the ones that do would wait for the others for good.
+    const int mine = wait(r) && !*abort_flag;
+    // These warps meet at a barrier below: they have to agree on whether to go on.
     int go;
-    {
-      const int mine = ok && !*abort_flag;
-      asm volatile(
-          "{\n\t.reg .pred P, Q;\n\tsetp.ne.s32 P, %1, 0;\n\tbarrier.cta.red.and.pred Q, 1, %2, P;\n\tselp.s32 %0, 1, 0, Q;\n\t}"
-          : "=r"(go)
-          : "r"(mine), "n"(32 * kWarps)
-          : "memory");
-    }
+    asm volatile(
+        "{\n\t.reg .pred P, Q;\n\tsetp.ne.s32 P, %1, 0;\n\tbarrier.cta.red.and.pred Q, 1, %2, P;\n\tselp.s32 %0, 1, 0, Q;\n\t}"
+        : "=r"(go)
+        : "r"(mine), "n"(32 * kW)
+        : "memory");
     if (!go) return;
     const Desc d = descs[r.stage];
     if (d.n_tiles == 0) return;
     // query rows as B operand: [k step][n tile][2]
-    uint32_t qf[8][kNB][2];
+    uint32_t qf[8][kNBS][2];
     {
-      const uint32_t base = ring0 + r.stage * kStageBytes + (lane & 7) * kPitch + d_quarter * 256 + (lane >> 3) * 16;
+      const uint32_t base = ring0 + r.stage * kStageBytes + (lane & 7) * kPitch + quarter * 256 + (lane >> 3) * 16;
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb)
+      for (int nb = 0; nb < kNBS; ++nb)
 #pragma unroll
         for (int ks = 0; ks < 8; ks += 2) {
           uint32_t x[4];
-          ldmatrix_x4(base + nb * 8 * kPitch + ks * 32, x);
+          ldmatrix_x4(base + (nb0 + nb) * 8 * kPitch + ks * 32, x);
           qf[ks][nb][0] = x[0], qf[ks][nb][1] = x[1], qf[ks + 1][nb][0] = x[2], qf[ks + 1][nb][1] = x[3];
         }
     }
-    release();
-    float o[kMT][kNB][4];
-#pragma unroll
-    for (int mt = 0; mt < kMT; ++mt)
-#pragma unroll
-      for (int nb = 0; nb < kNB; ++nb)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[mt][nb][e] = 0.f;
+    r.arrive_empty(lane);
+    r.next();
     // Query token i sees the keys [i + see_lo, i + see_hi) of the sequence's [0, len).
     const long long see_lo = p.win_left < 0 ? -(1ll << 40) : static_cast<long long>(d.len) - p.sq - p.win_left;
     const long long see_hi = p.win_right < 0 ? 1ll << 40 : static_cast<long long>(d.len) - p.sq + p.win_right + 1;
@@ -415,55 +466,54 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
 #pragma unroll
     for (int k = 0; k < kR; ++k) {
       m_row[k] = -INFINITY, l_row[k] = 0.f;
-      const int r = warp + kWarps * k, i = (d.row0 + r) / p.group;
+      const int row = warp + kW * k, i = (d.row0 + row) / p.group;
       if (lane == 0)  // only this warp reads its rows' bounds; rows that pad the block see nothing
-        bounds[r] = r < n_rows ? make_int2(static_cast<int>(max(0ll, i + see_lo)),
-                                           static_cast<int>(max(0ll, min(static_cast<long long>(d.len), i + see_hi))))
-                               : make_int2(0, 0);
+        bounds[row] = row < n_rows ? make_int2(static_cast<int>(max(0ll, i + see_lo)),
+                                               static_cast<int>(max(0ll, min(static_cast<long long>(d.len), i + see_hi))))
+                                   : make_int2(0, 0);
     }
     __syncwarp();
-
     // with key_weights: where the scores of this warp's rows go, and how many of their keys are counted
     const int counted = p.scores ? min(d.len, p.weights_len) : 0;
-    const int64_t score_pitch = static_cast<int64_t>(kWarps) * p.weights_len;
+    const int64_t score_pitch = static_cast<int64_t>(kW) * p.weights_len;
     float* const score_row =
         p.scores + (static_cast<int64_t>(d.b) * p.heads_kv * p.rows + d.head * p.rows + d.row0 + warp) * p.weights_len;
 
-    // partial scores of the tile in the ring's next stage: 16 keys x rows over a quarter of the head dimension
-    float s[kNB][4];
-    auto scores = [&]() {
+    for (int tile = 0; tile < d.n_tiles; ++tile) {
+      // ---- partial scores: 2 x 16 keys x rows
+      float s[2][kNBS][4];
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
-      wait_full();
-      const uint32_t base =
-          ring0 + r.stage * kStageBytes + (key_half * 16 + (lane & 15)) * kPitch + d_quarter * 256 + (lane >> 4) * 16;
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int ks = 0; ks < 8; ++ks) {
-        uint32_t a[4];
-        ldmatrix_x4(base + ks * 32, a);
+        for (int nb = 0; nb < kNBS; ++nb) s[h][nb][0] = s[h][nb][1] = s[h][nb][2] = s[h][nb][3] = 0.f;
+      wait(r);
+      const uint32_t base = ring0 + r.stage * kStageBytes + (lane & 15) * kPitch + quarter * 256 + (lane >> 4) * 16;
 #pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(s[nb], a, qf[ks][nb][0], qf[ks][nb][1]);
-      }
-      release();
-    };
-    auto put_scores = [&](int buf) {
-      float* part = part0 + buf * L::kPartFloats;
+      for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
-      for (int nb = 0; nb < kNB; ++nb) {
-        float* dst = part + (d_quarter * kRows + nb * 8 + frag_col) * kPartPitch + key_half * 16 + frag_row;
-        dst[0] = s[nb][0], dst[kPartPitch] = s[nb][1], dst[8] = s[nb][2], dst[kPartPitch + 8] = s[nb][3];
-      }
-    };
-    // softmax: a row at a time per warp, one key per lane
-    auto softmax = [&](int tile, int buf) {
-      const int key = d.first_key + tile * kTile + lane;
-      uint16_t* p_hi = reinterpret_cast<uint16_t*>(p0 + buf * 2 * L::kPWords);
-      uint16_t* p_lo = p_hi + 2 * L::kPWords;
-      // step by step over all rows, so that their latencies overlap
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a[4];
+          ldmatrix_x4(base + h * 16 * kPitch + ks * 32, a);
+#pragma unroll
+          for (int nb = 0; nb < kNBS; ++nb) mma_16816<kFp16>(s[h][nb], a, qf[ks][nb][0], qf[ks][nb][1]);
+        }
+      r.arrive_empty(lane);
+      r.next();
+      float* const part = part0 + (tile & 1) * L::kPartFloats;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int nb = 0; nb < kNBS; ++nb) {
+          float* dst = part + (quarter * kRows + (nb0 + nb) * 8 + frag_col) * kPartPitch + h * 16 + frag_row;
+          dst[0] = s[h][nb][0], dst[kPartPitch] = s[h][nb][1], dst[8] = s[h][nb][2], dst[kPartPitch + 8] = s[h][nb][3];
+        }
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kW) : "memory");
+      // ---- softmax: a row at a time, one key per lane; step by step over all rows, so that their latencies overlap
+      const int key0 = d.first_key + tile * kTile, key = key0 + lane;
       float x[kR], top[kR];
 #pragma unroll
       for (int k = 0; k < kR; ++k) {
-        const float* src = part0 + buf * L::kPartFloats + (warp + kWarps * k) * kPartPitch + lane;
+        const float* src = part + (warp + kW * k) * kPartPitch + lane;
         x[k] = (src[0] + src[kRows * kPartPitch]) + (src[2 * kRows * kPartPitch] + src[3 * kRows * kPartPitch]);
       }
       if (p.softcap > 0.f) {
@@ -473,25 +523,28 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
 #pragma unroll
         for (int k = 0; k < kR; ++k) x[k] *= scale_log2;
       }
-      const int key0 = d.first_key + tile * kTile;
       if (key0 < free_lo || key0 + kTile > free_hi) {
 #pragma unroll
         for (int k = 0; k < kR; ++k) {
-          const int2 vis = bounds[warp + kWarps * k];
+          const int2 vis = bounds[warp + kW * k];
           if (key < vis.x || key >= vis.y) x[k] = -INFINITY;
         }
       }
-#pragma unroll
-      for (int k = 0; k < kR; ++k) top[k] = warp_max(x[k]);
       if (key < counted) {
         float* to = score_row + key;
 #pragma unroll
         for (int k = 0; k < kR; ++k)
-          if (warp + kWarps * k < n_rows) to[k * score_pitch] = x[k];
+          if (warp + kW * k < n_rows) to[k * score_pitch] = x[k];
       }
 #pragma unroll
+      for (int k = 0; k < kR; ++k) top[k] = warp_max(x[k]);
+      rings.p.wait_empty(abort_flag, p.status, ST_TIMEOUT_SOFTMAX);
+      uint16_t* const p_hi = p0 + rings.p.stage * 4 * L::kPWords;
+      uint16_t* const p_lo = p_hi + 2 * L::kPWords;
+      float* const corr = corr0 + rings.p.stage * kRows;
+#pragma unroll
       for (int k = 0; k < kR; ++k) {
-        const int row = warp + kWarps * k;
+        const int row = warp + kW * k;
         const float m_new = fmaxf(m_row[k], top[k]);
         // a row that has seen no key yet: any finite reference gives p = 0 (and NaN for scores that are NaN)
         const float ref = m_new == -INFINITY ? 0.f : m_new;
@@ -501,13 +554,72 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
         uint16_t hi, lo;
         split16<kFp16>(e, hi, lo);
         p_hi[row * kPPitch * 2 + lane] = hi, p_lo[row * kPPitch * 2 + lane] = lo;
-        if (lane == 0) corr0[buf * kRows + row] = c;
+        if (lane == 0) corr[row] = c;
       }
-    };
-    // O^T += V^T P^T with the tile in the ring's next stage, a share of the head dimension's columns
-    auto values = [&](int buf) {
-      wait_full();
-      const float* corr = corr0 + buf * kRows;
+      rings.p.arrive_full(lane);
+      rings.p.next();
+    }
+    // ---- the stretch is done
+    rings.stat.wait_empty(abort_flag, p.status, ST_TIMEOUT_SOFTMAX);
+#pragma unroll
+    for (int k = 0; k < kR; ++k) {
+      float l = l_row[k];
+#pragma unroll
+      for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
+      const int row = warp + kW * k;
+      if (lane == 0) {
+        stat[row] = make_float2(m_row[k], l);
+        if (row < n_rows) {
+          const int unit_row = d.row0 + row;
+          if (d.slot < 0) {
+            const int i = unit_row / p.group, g = unit_row - i * p.group;
+            const float l2 = l == 0.f ? -INFINITY : m_row[k] + log2f(l);
+            if (p.lse) p.lse[(static_cast<int64_t>(d.b) * p.heads_q + d.head * p.group + g) * p.sq + i] = l2 * kLn2;
+            if (p.lse2) p.lse2[(static_cast<int64_t>(d.b) * p.heads_kv + d.head) * p.rows + unit_row] = l2;
+          } else {
+            p.part_ml[(blockIdx.x * 2 + d.slot) * p.rows_per_block + row] = make_float2(m_row[k], l);
+          }
+        }
+      }
+    }
+    rings.stat.arrive_full(lane);
+    rings.stat.next();
+  }
+}
+
+// Eight warps: O^T += V^T P^T, 64 columns of the head dimension each, behind the score warps. They do not wait for one
+// another, so one that gives up a wait just ends.
+template <bool kFp16, int kNB>
+__device__ __forceinline__ void value_warp(const PagedAttnParams& p, uint8_t* smem, Rings<kNB> rings, volatile int* abort_flag,
+                                           int warp, int lane) {
+  using L = Layout<kNB>;
+  constexpr int kRows = L::kRows;
+  constexpr int kMT = kHeadDim / kValueWarps / 16;  // 16-column tiles
+  const Desc* descs = reinterpret_cast<const Desc*>(smem + L::kOffDesc) + L::kKStages;
+  const uint32_t* p0 = reinterpret_cast<const uint32_t*>(smem + L::kOffP);
+  const float* corr0 = reinterpret_cast<const float*>(smem + L::kOffCorr);
+  const float2* stat = reinterpret_cast<const float2*>(smem + L::kOffStat);
+  auto& r = rings.v;
+  const uint32_t ring0 = smem_u32(smem) + L::kKStages * kStageBytes;
+  const int frag_row = lane >> 2, frag_col = (lane & 3) * 2;
+  auto wait = [&](const auto& ring) {
+    return __all_sync(0xffffffffu, ring.wait_full(abort_flag, p.status, ST_TIMEOUT_SOFTMAX));
+  };
+
+  while (true) {
+    if (!wait(r)) return;
+    const Desc d = descs[r.stage];
+    if (d.n_tiles == 0) return;
+    float o[kMT][kNB][4];
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+      for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[mt][nb][e] = 0.f;
+    for (int tile = 0; tile < d.n_tiles; ++tile) {
+      if (!wait(rings.p)) return;
+      const float* const corr = corr0 + rings.p.stage * kRows;
       float2 cf[kNB];
       bool any = false;
 #pragma unroll
@@ -524,65 +636,34 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
             o[mt][nb][2] *= cf[nb].x, o[mt][nb][3] *= cf[nb].y;
           }
       }
+      if (tile > 0 && !wait(r)) return;
       const uint32_t base =
           ring0 + r.stage * kStageBytes + ((lane & 7) + (lane >> 4) * 8) * kPitch + warp * (kMT * 32) + ((lane >> 3) & 1) * 16;
       // P as B operand, one load per k step and n tile: its upper numbers' two registers, then its lower ones'
-      const uint32_t p_base = smem_u32(p0 + (buf * 2 + (lane >> 4)) * L::kPWords) + (lane & 7) * (kPPitch * 4) + ((lane >> 3) & 1) * 16;
+      const uint32_t p_base =
+          smem_u32(p0 + (rings.p.stage * 2 + (lane >> 4)) * L::kPWords) + (lane & 7) * (kPPitch * 4) + ((lane >> 3) & 1) * 16;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
-        uint32_t a[kMT][4];
+        uint32_t pf[kNB][4];
 #pragma unroll
-        for (int mt = 0; mt < kMT; ++mt) ldmatrix_x4_trans(base + ks * 16 * kPitch + mt * 32, a[mt]);
+        for (int nb = 0; nb < kNB; ++nb) ldmatrix_x4(p_base + nb * 8 * kPPitch * 4 + ks * 32, pf[nb]);
 #pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) {
-          uint32_t pf[4];
-          ldmatrix_x4(p_base + nb * 8 * kPPitch * 4 + ks * 32, pf);
+        for (int mt = 0; mt < kMT; ++mt) {
+          uint32_t a[4];
+          ldmatrix_x4_trans(base + ks * 16 * kPitch + mt * 32, a);
 #pragma unroll
-          for (int mt = 0; mt < kMT; ++mt) mma_16816<kFp16>(o[mt][nb], a[mt], pf[0], pf[1]);
+          for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(o[mt][nb], a, pf[nb][0], pf[nb][1]);
 #pragma unroll
-          for (int mt = 0; mt < kMT; ++mt) mma_16816<kFp16>(o[mt][nb], a[mt], pf[2], pf[3]);
+          for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(o[mt][nb], a, pf[nb][2], pf[nb][3]);
         }
       }
-      release();
-    };
-    // One barrier per tile. Between two of them the warps have three independent things to do: the values of the tile
-    // before, the scores of the tile behind, and the softmax of this one.
-    scores();
-    put_scores(0);
-    sync();
-    for (int tile = 0; tile < d.n_tiles; ++tile) {
-      const int buf = tile & 1;
-      if (tile > 0) values(buf ^ 1);
-      const bool more = tile + 1 < d.n_tiles;
-      if (more) scores();
-      softmax(tile, buf);
-      if (more) put_scores(buf ^ 1);
-      sync();
+      r.arrive_empty(lane);
+      r.next();
+      rings.p.arrive_empty(lane);
+      rings.p.next();
     }
-    values((d.n_tiles - 1) & 1);
     // ---- the stretch is done
-#pragma unroll
-    for (int k = 0; k < kR; ++k) {
-      float l = l_row[k];
-#pragma unroll
-      for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
-      const int row = warp + kWarps * k;
-      if (lane == 0) {
-        stat[row] = make_float2(m_row[k], l);
-        const int unit_row = d.row0 + row;
-        if (row < p.rows_per_block && unit_row < p.rows) {
-          if (d.slot < 0) {
-            const int i = unit_row / p.group, g = unit_row - i * p.group;
-            const float l2 = l == 0.f ? -INFINITY : m_row[k] + log2f(l);
-            if (p.lse) p.lse[(static_cast<int64_t>(d.b) * p.heads_q + d.head * p.group + g) * p.sq + i] = l2 * kLn2;
-            if (p.lse2) p.lse2[(static_cast<int64_t>(d.b) * p.heads_kv + d.head) * p.rows + unit_row] = l2;
-          } else {
-            p.part_ml[(blockIdx.x * 2 + d.slot) * p.rows_per_block + row] = make_float2(m_row[k], l);
-          }
-        }
-      }
-    }
-    sync();
+    if (!wait(rings.stat)) return;
 #pragma unroll
     for (int nb = 0; nb < kNB; ++nb)
 #pragma unroll
@@ -607,34 +688,35 @@ __device__ __forceinline__ void consumer(const PagedAttnParams& p, uint8_t* smem
           for (int mt = 0; mt < kMT; ++mt) dst[mt * 16] = o[mt][nb][e], dst[mt * 16 + 8] = o[mt][nb][e + 2];
         }
       }
+    rings.stat.arrive_empty(lane);
+    rings.stat.next();
   }
 }
 
 template <bool kFp16, int kNB>
-__global__ void __launch_bounds__(kThreads, 1) splitd_paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
+__global__ void __launch_bounds__(kThreads<kNB>, 1) splitd_paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   using L = Layout<kNB>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffAbort);
-  Ring<L::kStages> r;
-  r.full = smem_u32(smem + L::kOffBar);
-  r.empty = r.full + 8 * L::kStages;
+  const Rings<kNB> rings(smem_u32(smem + L::kOffBar));
   if (threadIdx.x == 0) {
-    for (int i = 0; i < L::kStages; ++i) {
-      mbar_init(r.full + 8 * i, kProducers);
-      mbar_init(r.empty + 8 * i, kWarps);
-    }
+    rings.init();
     *abort_flag = 0;
     fence_mbar_init();
   }
   __syncthreads();
-  if (warp >= kWarps) {
-    if constexpr (kSplitRegs<kNB>) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs));
-    producer<kNB>(p, smem, r, abort_flag, warp - kWarps, lane);
+  if (warp >= kValueWarps + kScoreWarps<kNB>) {
+    if constexpr (kSplitRegs<kNB>) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProducerRegs<kNB>));
+    producer<kNB>(p, smem, rings, abort_flag, warp - kValueWarps - kScoreWarps<kNB>, lane);
+  } else if (warp >= kValueWarps) {
+    if constexpr (kSplitRegs<kNB>) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kScoreRegs<kNB>));
+    score_warp<kFp16, kNB>(p, smem, rings, abort_flag, warp - kValueWarps, lane);
   } else {
-    if constexpr (kSplitRegs<kNB>) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
-    consumer<kFp16, kNB>(p, smem, r, abort_flag, warp, lane);
+    if constexpr (kNB == 3) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kValueRegs<kNB>));
+    if constexpr (kNB == 4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kValueRegs<kNB>));
+    value_warp<kFp16, kNB>(p, smem, rings, abort_flag, warp, lane);
   }
 }
 
@@ -846,7 +928,7 @@ size_t paged_workspace_bytes(const splitd_paged_params* p) {
 namespace {
 
 template <typename Kernel>
-int raise_smem(Kernel kern, int bytes, int threads, bool split_regs, std::atomic<int> (&done)[64]) {
+int raise_smem(Kernel kern, int bytes, int threads, int split_total, std::atomic<int> (&done)[64]) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire)) return 0;
@@ -854,10 +936,10 @@ int raise_smem(Kernel kern, int bytes, int threads, bool split_regs, std::atomic
     cudaGetLastError();
     return fail(SPLITD_ERR_CUDA, "paged attention: the kernel's shared memory cannot be set");
   }
-  if (split_regs) {
+  if (split_total > 0) {
     cudaFuncAttributes at;
     if (cudaFuncGetAttributes(&at, kern) != cudaSuccess ||
-        at.numRegs * threads < 32 * pa::kProducers * pa::kProducerRegs + (threads - 32 * pa::kProducers) * pa::kConsumerRegs) {
+        at.numRegs * threads < split_total) {
       cudaGetLastError();
       return fail(SPLITD_ERR_CUDA, "paged attention: built with too few registers for its split");
     }
@@ -870,8 +952,8 @@ template <bool kFp16, int kNB>
 int launch_main(const PagedAttnParams& p, int grid, cudaStream_t stream) {
   static std::atomic<int> done[64];
   auto kern = pa::splitd_paged_attn_kernel<kFp16, kNB>;
-  if (int e = raise_smem(kern, pa::Layout<kNB>::kBytes, pa::kThreads, pa::kSplitRegs<kNB>, done)) return e;
-  kern<<<grid, pa::kThreads, pa::Layout<kNB>::kBytes, stream>>>(p);
+  if (int e = raise_smem(kern, pa::Layout<kNB>::kBytes, pa::kThreads<kNB>, pa::kSplitRegs<kNB> ? pa::kSplitTotal<kNB> : 0, done)) return e;
+  kern<<<grid, pa::kThreads<kNB>, pa::Layout<kNB>::kBytes, stream>>>(p);
   return 0;
 }
 
