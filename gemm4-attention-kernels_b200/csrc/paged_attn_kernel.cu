@@ -116,7 +116,6 @@ struct PagedAttnParams {
   int row_blocks, rows_per_block;
   int win_left, win_right;  // -1: unbounded
   float scale, softcap;
-  int min_tiles;   // a CTA takes at least this many tiles
   int max_ctas;
   // workspace
   float* part_o;   // [CTA][2][rows_per_block][512]
@@ -143,12 +142,17 @@ __device__ __forceinline__ int seq_tiles(const PagedAttnParams& p, int len) {
 }
 
 // The line of tiles: `total` over all sequences, cut into `ctas` shares; share c is [c total / ctas, (c+1) total / ctas).
+// A 64-bit division costs hundreds of cycles; most sizes fit 32 bits.
+__device__ __forceinline__ long long divide(long long a, long long b) {  // a >= 0, b > 0
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
 struct Line {
   long long total;
   int ctas;
   __device__ __forceinline__ long long begin(int c) const { return total * c / ctas; }
   __device__ __forceinline__ int owner(long long t) const {  // largest c with begin(c) <= t
-    return static_cast<int>(((t + 1) * ctas - 1) / total);
+    return static_cast<int>(divide((t + 1) * ctas - 1, total));
   }
 };
 __device__ __forceinline__ long long warp_sum(long long v) {
@@ -165,8 +169,7 @@ __device__ __forceinline__ long long tiles_before(const PagedAttnParams& p, int 
 __device__ __forceinline__ Line make_line(const PagedAttnParams& p, long long total) {
   Line ln;
   ln.total = total;
-  const long long want = (total + p.min_tiles - 1) / p.min_tiles;
-  ln.ctas = want < p.max_ctas ? static_cast<int>(want) : p.max_ctas;
+  ln.ctas = total < p.max_ctas ? static_cast<int>(total) : p.max_ctas;  // no more than tiles
   return ln;
 }
 
@@ -727,16 +730,16 @@ struct Span {
 };
 __device__ __forceinline__ Span span_of(const PagedAttnParams& p, int b, int lane) {
   long long before = 0, after = 0;
-  Span s;
-  s.n_tiles = 0, s.len = 0;
-  for (int i = lane; i < p.batch; i += 32) {
-    const int len = seq_len(p, i), t = seq_tiles(p, len);
-    if (i < b) before += t; else after += t;
-    if (i == b) s.n_tiles = t, s.len = len;
+#pragma unroll 4
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {  // the tiles of 32 sequences fit 32 bits
+    const int i = b0 + lane;
+    const unsigned t = i < p.batch ? seq_tiles(p, seq_len(p, i)) : 0u;
+    before += __reduce_add_sync(0xffffffffu, i < b ? t : 0u), after += __reduce_add_sync(0xffffffffu, i >= b ? t : 0u);
   }
   const int units = p.heads_kv * p.row_blocks;
-  s.first = warp_sum(before) * units, s.total = s.first + warp_sum(after) * units;
-  s.n_tiles = __shfl_sync(0xffffffffu, s.n_tiles, b & 31), s.len = __shfl_sync(0xffffffffu, s.len, b & 31);
+  Span s;
+  s.len = seq_len(p, b), s.n_tiles = seq_tiles(p, s.len);
+  s.first = before * units, s.total = (before + after) * units;
   return s;
 }
 // The CTAs [first, last] whose shares hold parts of a unit.
@@ -819,7 +822,9 @@ __device__ __forceinline__ void join_row(const PagedAttnParams& p, const Span& s
 template <int kThreads, bool kWide>
 __device__ __forceinline__ void add_weights(const PagedAttnParams& p, const Span& span, int b, int block) {
   constexpr int kRows = kWide ? 64 : kThreads;  // rows at a time
+  constexpr int kUnits = 64;
   __shared__ float lse2[kRows];
+  __shared__ int2 unit_owners[kWide ? kUnits : 1];  // of the sequence's first units
   const int tid = threadIdx.x, lane = tid & 31;
   const int n = min(span.len, p.weights_len);
   const int key0 = first_key(p, span.len) + block * kThreads;
@@ -831,6 +836,12 @@ __device__ __forceinline__ void add_weights(const PagedAttnParams& p, const Span
   }
   const int key = key0 + tid;
   const float* x = p.scores + static_cast<int64_t>(b) * rows * p.weights_len + key;
+  const int units = p.heads_kv * p.row_blocks;
+  if constexpr (kWide) {
+    for (int u = tid; u < min(units, kUnits); u += kThreads) unit_owners[u] = owners(p, span, u);
+    __syncthreads();
+    pdl_wait();
+  }
   float sum = 0.f;
   for (int r0 = 0; r0 < rows; r0 += kRows) {
     const int nr = min(kRows, rows - r0);
@@ -839,8 +850,9 @@ __device__ __forceinline__ void add_weights(const PagedAttnParams& p, const Span
       const int hr = r0 + r;
       const int head = hr / p.rows, unit_row = hr - head * p.rows;
       const int rb = unit_row / p.rows_per_block, row = unit_row - rb * p.rows_per_block;
-      const int2 own = owners(p, span, head * p.row_blocks + rb);
-      if (r0 == 0 && r == (kWide ? tid >> 5 : tid)) pdl_wait();
+      const int u = head * p.row_blocks + rb;
+      const int2 own = kWide && u < kUnits ? unit_owners[u] : owners(p, span, u);
+      if (!kWide) pdl_wait();
       float m = -INFINITY, l = 0.f;
       if (own.x == own.y) {
         m = p.lse2[static_cast<int64_t>(b) * rows + hr], l = 1.f;
@@ -862,7 +874,7 @@ __device__ __forceinline__ void add_weights(const PagedAttnParams& p, const Span
       }
       if (!kWide || lane == 0) lse2[r] = l == 0.f ? -INFINITY : m + log2f(l);
     }
-    if (r0 == 0) pdl_wait();
+    if (!kWide) pdl_wait();  // threads without a row
     __syncthreads();
     if (key < n) {
 #pragma unroll 16
@@ -906,7 +918,6 @@ int rows_per_block_of(int rows) { return (rows + row_blocks_of(rows) - 1) / row_
 
 int64_t max_keys(const splitd_paged_params* p) { return static_cast<int64_t>(p->max_pages) * p->page_size; }
 
-constexpr int kMinTiles = 1;
 constexpr int kMaxCtas = 256;  // sizes the workspace without asking a device
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
@@ -977,7 +988,6 @@ int launch_paged_attn(const splitd_paged_params* a, cudaStream_t stream) {
   p.win_left = a->local ? a->window_left : -1;
   p.win_right = a->causal ? 0 : a->local ? a->window_right : -1;
   p.scale = a->softmax_scale, p.softcap = a->softcap;
-  p.min_tiles = kMinTiles;
   p.status = a->status_flag;
   // no more CTAs than tiles there can be
   const int64_t most = static_cast<int64_t>(p.batch) * p.heads_kv * p.row_blocks * ((max_keys(a) + pa::kTile - 1) / pa::kTile);
@@ -1010,17 +1020,24 @@ int launch_paged_attn(const splitd_paged_params* a, cudaStream_t stream) {
   if (e) return e;
   cudaError_t ce = cudaGetLastError();
   // Few rows (so few units, each shared by many CTAs): four blocks a row, in which sixteen groups of threads read partial
-  // results side by side (1 x 131072 keys, 32 rows, 37 results each: 4 us, 7 us with one block of four groups a row). More
-  // rows: one small block each (8 x 230 keys, 512 rows, 8 results each: 12 us in
-  // all, 26 us the other way). The choice, which
-  // decides the order of the sums, does not look at the width of the page table.
-  const bool few = static_cast<int64_t>(p.batch) * p.heads_kv * p.rows <= sm_count();
+  // results side by side (1 x 131072 keys, 32 rows, 37 results each: 4 us, 7 us with one block of four groups a row). Eight
+  // results a row or more and up to two rows per SM: one block of four groups each (3 x 5452 keys, 192 rows: 27 us in all,
+  // 29 with small blocks; 8 x 230 keys, 512 rows: 16, 13). Otherwise one small block each. The choice, which decides the
+  // order of the sums, does not look at the width of the page table.
+  const int64_t units = static_cast<int64_t>(p.batch) * p.heads_kv * p.row_blocks;
+  const int64_t all_rows = static_cast<int64_t>(p.batch) * p.heads_kv * p.rows;
+  const bool few = all_rows <= sm_count();
+  const bool shared = units * 8 <= sm_count() && all_rows <= 2 * sm_count();
   const int64_t longest = !p.weights ? 0 : max_keys(a) < p.weights_len ? max_keys(a) : p.weights_len;
   const unsigned rows = p.heads_kv * p.rows;
   if (ce != cudaSuccess) {
   } else if (few) {
     const dim3 blocks(rows * 4 + static_cast<unsigned>((longest + 511) / 512), p.batch);
     ce = launch_dependent(fp16 ? pa::splitd_paged_finish_kernel<true, 16, 128> : pa::splitd_paged_finish_kernel<false, 16, 128>, blocks,
+                          dim3(512), 0, stream, p);
+  } else if (shared) {
+    const dim3 blocks(rows + static_cast<unsigned>((longest + 511) / 512), p.batch);
+    ce = launch_dependent(fp16 ? pa::splitd_paged_finish_kernel<true, 4, 512> : pa::splitd_paged_finish_kernel<false, 4, 512>, blocks,
                           dim3(512), 0, stream, p);
   } else {
     const dim3 blocks(rows + static_cast<unsigned>((longest + 127) / 128), p.batch);
