@@ -11,7 +11,7 @@
 // of 32-row stages (keys, values) full with one 1 KB bulk copy per row (a page of any size and a row of any page are then
 // the same thing: no tile has to match a page). One producer warp alone can issue such a copy every 74 cycles, 59 % of
 // the bandwidth. Measured: 1 x 131072 keys, 4 KV heads, 8 rows each: 158 us, 6.8 TB/s; 32 sequences of up to 8192: 207 us,
-// 6.7 TB/s (a plain copy moves 6.6). With 32 rows (4 tokens) a tile's instructions cost as much as its bytes: 103 us
+// 6.7 TB/s (a plain copy moves 6.6). With 32 rows (4 tokens) a tile's instructions cost as much as its bytes: 107 us
 // where the stream alone takes 94 and the bytes 81.
 //
 // Split. The (sequence, KV head, row block) units are laid end to end, in tiles of 32 keys, and every CTA takes an
@@ -91,7 +91,8 @@ struct Layout {
   static constexpr int kOffPart = kStages * kStageBytes;
   static constexpr int kOffP = kOffPart + 2 * kPartFloats * 4;
   static constexpr int kOffCorr = kOffP + 2 * 2 * kPWords * 4;
-  static constexpr int kOffStat = kOffCorr + 2 * kRows * 4;
+  static constexpr int kCorr = kRows + 4;  // factors of the rows, then whether some rows do not see some of the tile's keys
+  static constexpr int kOffStat = kOffCorr + 2 * kCorr * 4;
   static constexpr int kOffBounds = kOffStat + kRows * 8;
   static constexpr int kOffDesc = kOffBounds + kRows * 8;
   static constexpr int kOffBar = kOffDesc + kStages * static_cast<int>(sizeof(Desc));
@@ -187,6 +188,33 @@ __device__ __forceinline__ void split16(float p, uint16_t& hi, uint16_t& lo) {
     const __nv_bfloat16 h = __float2bfloat16_rz(below);
     hi = __bfloat16_as_ushort(h), lo = __bfloat16_as_ushort(__float2bfloat16_rn(p - __bfloat162float(h)));
   }
+}
+
+// Which keys the rows of a stretch of tiles see.
+struct Seen {
+  long long lo, hi;      // query token i: keys [i + lo, i + hi) of the sequence's [0, len)
+  int free_lo, free_hi;  // all rows of the block: keys [free_lo, free_hi)
+  int n_rows;
+  __device__ __forceinline__ Seen(const PagedAttnParams& p, const Desc& d) {
+    lo = p.win_left < 0 ? -(1ll << 40) : static_cast<long long>(d.len) - p.sq - p.win_left;
+    hi = p.win_right < 0 ? 1ll << 40 : static_cast<long long>(d.len) - p.sq + p.win_right + 1;
+    n_rows = min(p.rows_per_block, p.rows - d.row0);
+    free_lo = first((d.row0 + n_rows - 1) / p.group);
+    free_hi = end(d.row0 / p.group, d.len);
+  }
+  __device__ __forceinline__ int first(int i) const { return static_cast<int>(max(0ll, i + lo)); }
+  __device__ __forceinline__ int end(int i, int len) const {
+    return static_cast<int>(max(0ll, min(static_cast<long long>(len), i + hi)));
+  }
+  // whether every row of the block sees every key of the tile
+  __device__ __forceinline__ bool all_of(int key0) const { return key0 >= free_lo && key0 + kTile <= free_hi; }
+};
+
+// whether one of two 16-bit numbers is an infinity or NaN
+template <bool kFp16>
+__device__ __forceinline__ bool not_finite2(uint32_t x) {
+  constexpr uint32_t kExp = kFp16 ? 0x7c00u : 0x7f80u;
+  return (x & kExp) == kExp || (x >> 16 & kExp) == kExp;
 }
 
 // largest value of the warp in all lanes; NaN are passed over
@@ -458,22 +486,14 @@ __device__ __forceinline__ void score_warp(const PagedAttnParams& p, uint8_t* sm
     }
     r.arrive_empty(lane);
     r.next();
-    // Query token i sees the keys [i + see_lo, i + see_hi) of the sequence's [0, len).
-    const long long see_lo = p.win_left < 0 ? -(1ll << 40) : static_cast<long long>(d.len) - p.sq - p.win_left;
-    const long long see_hi = p.win_right < 0 ? 1ll << 40 : static_cast<long long>(d.len) - p.sq + p.win_right + 1;
-    const int n_rows = min(p.rows_per_block, p.rows - d.row0);
-    // keys that all rows of the block see: tiles inside need no mask
-    const int free_lo = static_cast<int>(max(0ll, (d.row0 + n_rows - 1) / p.group + see_lo));
-    const int free_hi = static_cast<int>(max(0ll, min(static_cast<long long>(d.len), d.row0 / p.group + see_hi)));
+    const Seen seen(p, d);
     float m_row[kR], l_row[kR];
 #pragma unroll
     for (int k = 0; k < kR; ++k) {
       m_row[k] = -INFINITY, l_row[k] = 0.f;
       const int row = warp + kW * k, i = (d.row0 + row) / p.group;
       if (lane == 0)  // only this warp reads its rows' bounds; rows that pad the block see nothing
-        bounds[row] = row < n_rows ? make_int2(static_cast<int>(max(0ll, i + see_lo)),
-                                               static_cast<int>(max(0ll, min(static_cast<long long>(d.len), i + see_hi))))
-                                   : make_int2(0, 0);
+        bounds[row] = row < seen.n_rows ? make_int2(seen.first(i), seen.end(i, d.len)) : make_int2(0, 0);
     }
     __syncwarp();
     // with key_weights: where the scores of this warp's rows go, and how many of their keys are counted
@@ -526,7 +546,7 @@ __device__ __forceinline__ void score_warp(const PagedAttnParams& p, uint8_t* sm
 #pragma unroll
         for (int k = 0; k < kR; ++k) x[k] *= scale_log2;
       }
-      if (key0 < free_lo || key0 + kTile > free_hi) {
+      if (!seen.all_of(key0)) {
 #pragma unroll
         for (int k = 0; k < kR; ++k) {
           const int2 vis = bounds[warp + kW * k];
@@ -537,14 +557,14 @@ __device__ __forceinline__ void score_warp(const PagedAttnParams& p, uint8_t* sm
         float* to = score_row + key;
 #pragma unroll
         for (int k = 0; k < kR; ++k)
-          if (warp + kW * k < n_rows) to[k * score_pitch] = x[k];
+          if (warp + kW * k < seen.n_rows) to[k * score_pitch] = x[k];
       }
 #pragma unroll
       for (int k = 0; k < kR; ++k) top[k] = warp_max(x[k]);
       rings.p.wait_empty(abort_flag, p.status, ST_TIMEOUT_SOFTMAX);
       uint16_t* const p_hi = p0 + rings.p.stage * 4 * L::kPWords;
       uint16_t* const p_lo = p_hi + 2 * L::kPWords;
-      float* const corr = corr0 + rings.p.stage * kRows;
+      float* const corr = corr0 + rings.p.stage * L::kCorr;
 #pragma unroll
       for (int k = 0; k < kR; ++k) {
         const int row = warp + kW * k;
@@ -559,6 +579,7 @@ __device__ __forceinline__ void score_warp(const PagedAttnParams& p, uint8_t* sm
         p_hi[row * kPPitch * 2 + lane] = hi, p_lo[row * kPPitch * 2 + lane] = lo;
         if (lane == 0) corr[row] = c;
       }
+      if (warp == 0 && lane == 0) corr[kRows] = key0 < seen.free_lo || min(key0 + kTile, d.len) > seen.free_hi ? 1.f : 0.f;
       rings.p.arrive_full(lane);
       rings.p.next();
     }
@@ -572,7 +593,7 @@ __device__ __forceinline__ void score_warp(const PagedAttnParams& p, uint8_t* sm
       const int row = warp + kW * k;
       if (lane == 0) {
         stat[row] = make_float2(m_row[k], l);
-        if (row < n_rows) {
+        if (row < seen.n_rows) {
           const int unit_row = d.row0 + row;
           if (d.slot < 0) {
             const int i = unit_row / p.group, g = unit_row - i * p.group;
@@ -622,7 +643,7 @@ __device__ __forceinline__ void value_warp(const PagedAttnParams& p, uint8_t* sm
         for (int e = 0; e < 4; ++e) o[mt][nb][e] = 0.f;
     for (int tile = 0; tile < d.n_tiles; ++tile) {
       if (!wait(rings.p)) return;
-      const float* const corr = corr0 + rings.p.stage * kRows;
+      const float* const corr = corr0 + rings.p.stage * L::kCorr;
       float2 cf[kNB];
       bool any = false;
 #pragma unroll
@@ -645,19 +666,59 @@ __device__ __forceinline__ void value_warp(const PagedAttnParams& p, uint8_t* sm
       // P as B operand, one load per k step and n tile: its upper numbers' two registers, then its lower ones'
       const uint32_t p_base =
           smem_u32(p0 + (rings.p.stage * 2 + (lane >> 4)) * L::kPWords) + (lane & 7) * (kPPitch * 4) + ((lane >> 3) & 1) * 16;
+      // Where some rows do not see some keys, an infinity or NaN among those keys' values must not reach them through a
+      // weight of 0 (0 * inf). Such tiles are few, and such values next to none.
+      bool products = true;
+      if (corr[kRows] != 0.f) {
+        bool bad = false;
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        uint32_t pf[kNB][4];
-#pragma unroll
-        for (int nb = 0; nb < kNB; ++nb) ldmatrix_x4(p_base + nb * 8 * kPPitch * 4 + ks * 32, pf[nb]);
-#pragma unroll
-        for (int mt = 0; mt < kMT; ++mt) {
+        for (int i = 0; i < 2 * kMT; ++i) {
           uint32_t a[4];
-          ldmatrix_x4_trans(base + ks * 16 * kPitch + mt * 32, a);
+          ldmatrix_x4_trans(base + (i & 1) * 16 * kPitch + (i >> 1) * 32, a);
+          bad |= not_finite2<kFp16>(a[0]) || not_finite2<kFp16>(a[1]) || not_finite2<kFp16>(a[2]) || not_finite2<kFp16>(a[3]);
+        }
+        products = !__any_sync(0xffffffffu, bad);
+      }
+      if (products) {
 #pragma unroll
-          for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(o[mt][nb], a, pf[nb][0], pf[nb][1]);
+        for (int ks = 0; ks < 2; ++ks) {
+          uint32_t pf[kNB][4];
 #pragma unroll
-          for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(o[mt][nb], a, pf[nb][2], pf[nb][3]);
+          for (int nb = 0; nb < kNB; ++nb) ldmatrix_x4(p_base + nb * 8 * kPPitch * 4 + ks * 32, pf[nb]);
+#pragma unroll
+          for (int mt = 0; mt < kMT; ++mt) {
+            uint32_t a[4];
+            ldmatrix_x4_trans(base + ks * 16 * kPitch + mt * 32, a);
+#pragma unroll
+            for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(o[mt][nb], a, pf[nb][0], pf[nb][1]);
+#pragma unroll
+            for (int nb = 0; nb < kNB; ++nb) mma_16816<kFp16>(o[mt][nb], a, pf[nb][2], pf[nb][3]);
+          }
+        }
+      } else {
+        const uint8_t* v_at = smem + L::kKStages * kStageBytes + r.stage * kStageBytes + (warp * (kMT * 16) + frag_row) * 2;
+        const uint16_t* p_at = reinterpret_cast<const uint16_t*>(p0 + rings.p.stage * 2 * L::kPWords) + frag_col * kPPitch * 2;
+#pragma unroll 1
+        for (int key = 0; key < kTile; ++key) {
+          float unused;
+#pragma unroll
+          for (int nb = 0; nb < kNB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const volatile uint16_t* at = p_at + (nb * 8 + e) * kPPitch * 2 + key;
+              float hi, lo;
+              unpack2<kFp16>(at[0], hi, unused);
+              unpack2<kFp16>(at[2 * L::kPWords], lo, unused);
+              const float w = hi + lo;
+              if (w != 0.f) {
+#pragma unroll
+                for (int i = 0; i < 2 * kMT; ++i) {
+                  float v;
+                  unpack2<kFp16>(*reinterpret_cast<const volatile uint16_t*>(v_at + key * kPitch + i * 16), v, unused);
+                  o[i >> 1][nb][e + 2 * (i & 1)] += w * v;
+                }
+              }
+            }
         }
       }
       r.arrive_empty(lane);

@@ -251,8 +251,7 @@ def split_flash_attn_paged_func(
     its Sq new tokens: query i stands at slot ``seqlens_k[b] - Sq + i``, and ``causal``, ``window_size`` and ``softcap``
     mean what they mean in ``split_flash_attn_func`` (bottom-right alignment; causal changes nothing for Sq = 1). A row
     that sees no slot, as in a sequence of length 0, gets out 0 and lse -inf. Slots that no row of a sequence may see
-    are not read; one that only some of its rows may see has weight 0 in the others, like any masked key of a dense
-    product (0 times an infinity is NaN there too).
+    are not read, and one that only some rows may see leaves the others alone, whatever it holds.
 
     ``key_weights`` (B, slots) float32, optional: every slot's softmax weight, summed over all query heads and tokens,
     is added to it in place, in a fixed order (what ``split_paged_evict_func`` ranks by). Costs a workspace of

@@ -229,7 +229,8 @@ size_t splitd_bwd_static_scratch_limit_workspace(void); /* 16 MiB         */
 /* Attention of seqlen_q query tokens per sequence (one when decoding, a few when verifying drafted ones) over the
  * cache. seqlens_k[b] counts the slots of sequence b with the new tokens in it: query i stands at slot
  * seqlens_k[b] - seqlen_q + i, which is where causal and the window are measured from. Rows without a visible key get
- * o = 0 and lse = -inf; slots that no query row of the sequence may see are not read at all. */
+ * o = 0 and lse = -inf; slots that no query row of the sequence may see are not read at all, and infinities or NaN in
+ * one that only some rows may see do not reach the others. */
 typedef struct {
   const void* q;       /* (B, Sq, Hq, 512) */
   const void* k_pages; /* (num_pages, page_size, Hkv, 512) */

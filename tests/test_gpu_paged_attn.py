@@ -143,6 +143,40 @@ def test_nan_and_infinity_of_a_visible_key_reach_the_rows_that_see_it_only():
     assert_status_ok()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,sq", [((8, 1), 2), ((8, 2), 4), ((8, 1), 3), ((8, 1), 4), ((4, 4), 40)])
+def test_infinities_and_nan_in_keys_that_only_some_rows_see(dtype, heads, sq):
+    """Drafted tokens: the last slots are hidden from the first rows, whose results must not notice what is in them."""
+    from splitd_flash_attn import split_flash_attn_paged_func
+
+    lens = [70, 33, sq, 200]
+    k, v, table, seqlens, _ = make_cache(lens, 16, heads[1], dtype, 13)
+    q = make_q(4, sq, heads[0], dtype, 13)
+    for mask in ({"causal": True}, {"window_size": (20, 0)}):
+        clean, clean_lse = split_flash_attn_paged_func(q, k, v, table, seqlens, return_lse=True, **mask)
+        k2, v2 = k.clone(), v.clone()
+        for b, n in enumerate(lens):
+            last = table[b, (n - 1) // 16].long(), (n - 1) % 16
+            k2[last], v2[last] = float("nan"), float("nan")
+        out, lse = split_flash_attn_paged_func(q, k2, v2, table, seqlens, return_lse=True, **mask)
+        assert torch.equal(lse[:, :, :-1], clean_lse[:, :, :-1]) and torch.isnan(lse[:, :, -1]).all()
+        # a tile with such a value is summed one key at a time: other roundings of the same sum of 32 terms
+        seen = torch.isfinite(clean_lse).transpose(1, 2)[:, :-1, :, None]
+        diff = (out[:, :-1].double() - clean[:, :-1].double()).abs()
+        assert torch.isfinite(out[:, :-1]).all() and torch.isnan(out[:, -1]).all()
+        bound = torch.finfo(dtype).eps * clean[:, :-1].double().abs() + 64 * 2.0**-23 * v.abs().nan_to_num(0).amax().double()
+        assert (diff <= bound * seen + 0.0).all()
+        v2 = v.clone()
+        for b, n in enumerate(lens):
+            v2[table[b, (n - 1) // 16].long(), (n - 1) % 16, :, 5] = float("inf")
+        out = split_flash_attn_paged_func(q, k, v2, table, seqlens, **mask)
+        assert torch.isfinite(out[:, :-1]).all() and (out[:, -1, :, 5] == float("inf")).all()
+        rest = torch.ones(D, dtype=torch.bool, device="cuda")
+        rest[5] = False
+        assert torch.isfinite(out[:, -1][..., rest]).all()
+    assert_status_ok()
+
+
 def test_strided_caches_and_queries():
     """Keys and values interleaved in one allocation, heads before rows, a slice of a larger q."""
     from splitd_flash_attn import split_flash_attn_paged_func

@@ -466,3 +466,22 @@ def test_on_a_stream_of_its_own():
     for g in got:
         assert all(torch.equal(a, b) for a, b in zip(want, g))
     assert_status_ok()
+
+
+def test_custom_ops_keep_their_schemas():
+    """What torch checks of a custom op: aliasing and mutation as declared, fake kernels, autograd, dynamic shapes."""
+    ops = torch.ops.splitd_flash_attn
+    k, v, table, seqlens, free = make_cache([40, 21], 16, 2, torch.bfloat16, 23, spare=4, fill=0.0)
+    q, kk = tokens((2, 1), 8, torch.bfloat16, 1), tokens((2, 1), 2, torch.bfloat16, 2)
+    w, f, none, pos = torch.rand(2, 40, device="cuda"), freq(512), -(2**31), torch.arange(1, device="cuda")
+    for op, args in (
+        (ops.paged_attn, (q, k, v, table, seqlens, w, 0.05, True, none, none, 0.0)),
+        (ops.paged_attn, (q, k, v, table, seqlens, None, 0.05, False, 5, 0, 20.0)),
+        (ops.paged_append, (q, kk, kk, k, v, table, seqlens, f, None, None, False, 1.0)),
+        (ops.paged_append, (None, kk, kk, k, v, table, seqlens, None, None, None, False, 1.0)),
+        (ops.paged_evict, (k, v, table, seqlens, w, free[:4].view(2, 2), 20, 2, 2)),
+        (ops.rotary, (q.clone().requires_grad_(), kk.clone().requires_grad_(), pos, f, False, 1.0, False)),
+        (ops.rotary, (None, kk, pos, f, True, 1.0, True)),
+    ):
+        torch.library.opcheck(op.default, args)
+    assert_status_ok()
