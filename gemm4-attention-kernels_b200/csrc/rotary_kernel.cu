@@ -12,7 +12,9 @@
 //
 // What bounds it. 2 bytes in and 2 out per element, a handful of operations: HBM. One warp takes a token and a run of
 // its heads; a lane holds the two 16-byte pieces of a head row that belong together, so that both halves of a pair are
-// in its registers, and asks for four head rows before it uses the first.
+// in its registers, and asks for four head rows before it uses the first. Measured: 2 x 8192 tokens, 36 heads: 193 us a
+// direction, 6.2 TB/s, 95 % of a plain copy's rate (212 us where the halves start at no 16-byte boundary and rows go
+// through shared memory); 24576 tokens into a cache, 40 heads: 229 us, 6.3 TB/s.
 #include <cstring>
 
 #include "launch.cuh"
