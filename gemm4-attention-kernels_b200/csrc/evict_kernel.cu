@@ -12,7 +12,7 @@
 // A cluster of eight CTAs per sequence, each with its share of the slots; histograms and counts meet through distributed
 // shared memory. Up to kOneCta slots a single CTA is faster than the cluster's barriers. The weights are read once and
 // their keys kept in shared memory (a sequence of more than eight times kCacheMost slots is read from L2 again). What
-// bounds it is the chain of passes and barriers (131072 slots: 19 us; the copy of 20000 of them, 4 heads: 50 us), not
+// bounds it is the chain of passes and barriers (131072 slots: 18 us; the copy of 20000 of them, 4 heads: 50 us), not
 // bytes.
 //
 // Copy. The kept slots' head rows are laid end to end; a warp takes four of them of one tensor, whose places four of its
@@ -71,7 +71,7 @@ __device__ __forceinline__ int cache_len(const EvictParams& p, int len) {
 }
 
 template <int kCtas>
-__global__ void __launch_bounds__(kThreads) splitd_evict_select_kernel(const __grid_constant__ EvictParams p) {
+__global__ void __launch_bounds__(kThreads, 1) splitd_evict_select_kernel(const __grid_constant__ EvictParams p) {
   extern __shared__ uint32_t cache[];  // keys of this CTA's slots
   namespace cg = cooperative_groups;
   __shared__ unsigned hist[kBins];   // of this CTA
@@ -93,26 +93,21 @@ __global__ void __launch_bounds__(kThreads) splitd_evict_select_kernel(const __g
     cluster.sync();
     const int* first = cluster.map_shared_rank(length, 0);
     stated = first[0], n = first[1];
-    cluster.sync();  // no CTA ends while another may read its memory
   } else {
     __syncthreads();
     stated = length[0], n = length[1];
   }
   const int m = min(n, p.keep);
-  if (gtid == 0) {
-    p.new_seqlens[b] = m;
-    if (p.status && stated > n) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
-  }
+  if (gtid == 0 && p.status && stated > n) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
   int* kept = p.kept + static_cast<int64_t>(b) * p.keep;
-  for (int i = m + gtid; i < p.keep; i += step) kept[i] = -1;
   if (n <= p.keep) {  // the whole cluster: everything stays
-    for (int i = gtid; i < n; i += step) kept[i] = i;
+    for (int i = gtid; i < p.keep; i += step) kept[i] = i < n ? i : -1;
+    if (gtid == 0) p.new_seqlens[b] = m;
+    if constexpr (kCtas > 1) cluster.sync();  // no CTA ends while another may read its memory
     return;
   }
   // slots in [lo, hi) compete for the places that the first and the recent ones leave
   const int lo = p.keep_first, hi = n - p.keep_recent;
-  for (int i = gtid; i < lo; i += step) kept[i] = i;
-  for (int i = hi + gtid; i < n; i += step) kept[m - (n - i)] = i;
   const float* w = p.weights + b * p.weights_stride;
   const int per = ((hi - lo) + kCtas - 1) / kCtas;
   const int c0 = min(lo + rank * per, hi), c1 = min(c0 + per, hi);
@@ -231,6 +226,10 @@ __global__ void __launch_bounds__(kThreads) splitd_evict_select_kernel(const __g
 #pragma unroll 4
     for (int i0 = w0; i0 < w1; i0 += 32) place(i0 + lane, i0 + lane < w1 ? order_key(__ldg(w + c0 + i0 + lane)) : 0u);
   }
+  // the first and the recent ones; not before the barriers, which would wait for the stores
+  for (int i = gtid; i < lo; i += step) kept[i] = i;
+  for (int i = hi + gtid; i < n; i += step) kept[m - (n - i)] = i;
+  if (gtid == 0) p.new_seqlens[b] = m;
   if constexpr (kCtas > 1) cluster.barrier_wait();  // no CTA ends while another may read its memory
 }
 
