@@ -293,7 +293,7 @@ def test_evict_function_checks(fake):
         fn(k, v, t, n, w, new.long(), 4)
     with pytest.raises(ValueError, match="key_weights"):
         fn(k, v, t, n, w[0], new, 4)
-    with pytest.raises(ValueError, match="2\^30"):
+    with pytest.raises(ValueError, match=r"2\^30"):
         fn(k, v, t, n, w, new, 2**30 + 1)
     with pytest.raises(ValueError, match="expanded"):
         fn(k[:1].expand(10, -1, -1, -1), v, t, n, w, new, 4)
