@@ -379,6 +379,7 @@ __device__ __forceinline__ void producer(const PagedAttnParams& p, uint8_t* smem
           fence_proxy_async_smem();
         }
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, have)) * kRowBytes;
+        __syncwarp();  // all lanes' zeros before the arrival that hands the stage over (a ballot orders no memory)
         if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
         __syncwarp();
         if (have) bulk_load(dst, src, kRowBytes, bar);
