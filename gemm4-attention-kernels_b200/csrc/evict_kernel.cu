@@ -247,7 +247,10 @@ __global__ void __launch_bounds__(kCopyWarps * 32) splitd_evict_copy_kernel(cons
   pdl_wait();
   if (lane < kCopyRows && place < p.keep) {
     const int64_t at = static_cast<int64_t>(b) * p.keep + place;
-    const int slot = p.kept[at];
+    // `kept` has a hole (what its memory held before) if somebody changed the weights during the selection of a sequence
+    // whose keys do not fit in shared memory; what is no slot of this cache is not followed.
+    int slot = p.kept[at];
+    if (slot >= min(page_capacity(p.from), p.weights_len)) slot = -1;
     if (h == 0 && !is_v) p.new_weights[at] = slot < 0 ? 0.f : __ldg(p.weights + b * p.weights_stride + slot);
     if (slot >= 0) {
       int entry, in_page;
