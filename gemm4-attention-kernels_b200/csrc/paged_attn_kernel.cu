@@ -24,9 +24,14 @@
 // partial sums meet in shared memory, where score warp w then owns the softmax of every fourth (eighth) row, one key per
 // lane. O^T = V^T P^T is split over the head dimension, 64 columns per value warp, accumulators in registers. Score and
 // value warps only meet through two buffers of P, so that products and softmax of neighbouring tiles overlap (one set of
-// eight warps for both, with one barrier a tile: 119 us with 32 rows, 103 us this way; up to 24 rows the same). P is kept
-// as the sum of TWO 16-bit numbers (two products): a single one would put an error of the size of the output's own
-// rounding on top of it.
+// eight warps for both, with one barrier a tile: 119 us with 32 rows, 103 us this way; up to 24 rows the same).
+//
+// Roundings. The matrix instruction multiplies V, which is exact, by P in V's 16-bit type. P is kept as the sum of TWO such
+// numbers (two products): a single one would put an error of the size of the output's own rounding on top of it. Two
+// leave a weight off by 2^-16 of itself in bf16 and by 2^-22 in fp16, a 128th and a 1024th of the output's rounding; three
+// would cost a third product for an error that the scores' own sums in 32 bits have as well. The weights are at most 1, and
+// fp16 ends at 2^-24, so there P is 2^16 times the weight, taken out again where l divides: what a weight loses is then at
+// most 2^-41 of the row's largest one (without the factor, 131071 keys at 2^-26 of one whose value is 0 came out as 0).
 #include <cstring>
 
 #include "launch.cuh"
@@ -119,7 +124,7 @@ struct PagedAttnParams {
   float scale, softcap;
   int max_ctas;
   // workspace
-  float* part_o;   // [CTA][2][rows_per_block][512]
+  float* part_o;   // [CTA][2][rows_per_block][512], kPScale times O
   float2* part_ml; // [CTA][2][rows_per_block]
   float* lse2;     // [batch][heads_kv * rows] in log2 units, of the rows that one CTA finished; only with key_weights
   float* scores;   // [batch][heads_kv * rows][weights_len], only with key_weights
@@ -176,8 +181,16 @@ __device__ __forceinline__ Line make_line(const PagedAttnParams& p, long long to
 
 namespace pa {
 
+// What P is multiplied by, a power of two: 2^16 is the largest whose product with a weight of 1 two fp16 numbers hold
+// (65504 + 32).
+template <bool kFp16>
+constexpr float kPScale = kFp16 ? 65536.f : 1.f;
+template <bool kFp16>
+constexpr float kPUnscale = 1.f / kPScale<kFp16>;
+
 // p >= 0 as a sum of two 16-bit numbers. The upper one is the largest that is LESS than p, so that both are positive
-// where p is: a visible infinity of V times p stays an infinity (inf * 0 and inf - inf would be NaN).
+// where p is: a visible infinity of V times p stays an infinity (inf * 0 and inf - inf would be NaN). In fp16 that ends
+// at p = 2^-24, a weight of 2^-40 of the largest.
 template <bool kFp16>
 __device__ __forceinline__ void split16(float p, uint16_t& hi, uint16_t& lo) {
   const float below = p > 0.f ? __uint_as_float(__float_as_uint(p) - 1) : p;
@@ -576,7 +589,7 @@ __device__ __forceinline__ void score_warp(const PagedAttnParams& p, uint8_t* sm
         m_row[k] = m_new;
         l_row[k] = l_row[k] * c + e;
         uint16_t hi, lo;
-        split16<kFp16>(e, hi, lo);
+        split16<kFp16>(e * kPScale<kFp16>, hi, lo);
         p_hi[row * kPPitch * 2 + lane] = hi, p_lo[row * kPPitch * 2 + lane] = lo;
         if (lane == 0) corr[row] = c;
       }
@@ -740,7 +753,7 @@ __device__ __forceinline__ void value_warp(const PagedAttnParams& p, uint8_t* sm
         if (d.slot < 0) {
           const int i = unit_row / p.group, g = unit_row - i * p.group;
           const float l = stat[row].y;
-          const float inv = l == 0.f ? 0.f : 1.f / l;
+          const float inv = l == 0.f ? 0.f : kPUnscale<kFp16> / l;
           uint16_t* dst = p.o + d.b * p.o_sb + i * p.o_ss + (d.head * p.group + g) * p.o_sh + col;
 #pragma unroll
           for (int mt = 0; mt < kMT; ++mt) {
@@ -871,7 +884,7 @@ __device__ __forceinline__ void join_row(const PagedAttnParams& p, const Span& s
       s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : kPUnscale<kFp16> / l;
   uint2 w;
   w.x = pack2<kFp16>(s.x * inv, s.y * inv), w.y = pack2<kFp16>(s.z * inv, s.w * inv);
   *reinterpret_cast<uint2*>(out + col) = w;
