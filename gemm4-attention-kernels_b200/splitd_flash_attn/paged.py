@@ -124,7 +124,8 @@ def _check_weights(key_weights, batch, device) -> None:
 
 
 def _unit_rows(*tensors) -> bool:
-    return all(t.stride(-1) == 1 or t.shape[-1] < 2 for t in tensors)
+    # of a tensor without elements contiguous() would not change the strides
+    return all(t.stride(-1) == 1 or t.shape[-1] < 2 or t.numel() == 0 for t in tensors)
 
 
 # ---------------------------------------------------------------------------
