@@ -118,9 +118,21 @@ def _token_strides(t: torch.Tensor):
     return s[:3] if t.ndim == 4 else (0, s[0], s[1])
 
 
+# Dispatch keys that every thread includes; any other belongs to something that wants to see each operator.
+_USUAL_KEYS = (
+    torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect) | torch._C.DispatchKeySet(torch._C.DispatchKey.ADInplaceOrView)
+).raw_repr()
+
+
 def _traced(*tensors) -> bool:
-    """Whether the call goes through its custom op: under torch.compile, and for tensors without memory."""
-    return torch.compiler.is_compiling() or any(t is not None and type(t) is not torch.Tensor for t in tensors)
+    """Whether the call goes through its custom op: under torch.compile, for tensors without memory and other subclasses, and
+    where a tracer, a dispatch mode or a function transform is at work. Otherwise the kernel is called without the
+    dispatcher, which costs several times what the kernels of a decode step take."""
+    return (
+        torch.compiler.is_compiling()
+        or bool(torch._C._dispatch_tls_local_include_set().raw_repr() & ~_USUAL_KEYS)
+        or any(t is not None and type(t) is not torch.Tensor for t in tensors)
+    )
 
 
 # ---------------------------------------------------------------------------
@@ -272,8 +284,7 @@ class RotaryFunc(torch.autograd.Function):
             dk = None
         if dq is None and dk is None:
             return (None,) * 7
-        run = RotaryFunc.apply if torch.is_grad_enabled() else _rotary
-        dq, dk = run(dq, dk, positions, inv_freq, interleaved, factor, not backward)
+        dq, dk = _turned(dq, dk, positions, inv_freq, interleaved, factor, not backward)
         return dq, dk, None, None, None, None, None
 
 
@@ -319,6 +330,16 @@ def _rotary_backward(ctx, dq, dk):
 torch.library.register_autograd("splitd_flash_attn::rotary", _rotary_backward, setup_context=_rotary_setup_context)
 
 
+def _turned(q, k, positions, inv_freq, interleaved, factor, backward):
+    if _traced(q, k):
+        _check_rotary(q, k, positions, inv_freq)
+        q_out, k_out = torch.ops.splitd_flash_attn.rotary(q, k, positions, inv_freq, interleaved, factor, backward)
+        return (None if q is None else q_out), (None if k is None else k_out)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
+        return RotaryFunc.apply(q, k, positions, inv_freq, interleaved, factor, backward)
+    return _rotary(q, k, positions, inv_freq, interleaved, factor, backward)
+
+
 def split_rotary_func(
     q: Optional[torch.Tensor],
     k: Optional[torch.Tensor],
@@ -336,11 +357,4 @@ def split_rotary_func(
     far positions lose nothing. A pair is dimensions (i, i + rotary_dim / 2), with ``interleaved`` (2 i, 2 i + 1).
     ``factor`` scales what is rotated; the dimensions behind pass through unchanged.
     """
-    interleaved, factor = bool(interleaved), float(factor)
-    if _traced(q, k):
-        _check_rotary(q, k, positions, inv_freq)
-        q_out, k_out = torch.ops.splitd_flash_attn.rotary(q, k, positions, inv_freq, interleaved, factor, False)
-        return (None if q is None else q_out), (None if k is None else k_out)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
-        return RotaryFunc.apply(q, k, positions, inv_freq, interleaved, factor, False)
-    return _rotary(q, k, positions, inv_freq, interleaved, factor, False)
+    return _turned(q, k, positions, inv_freq, bool(interleaved), float(factor), False)
