@@ -128,6 +128,11 @@ def _unit_rows(*tensors) -> bool:
     return all(t.stride(-1) == 1 or t.shape[-1] < 2 or t.numel() == 0 for t in tensors)
 
 
+def _written(*tensors) -> None:
+    """For autograd, as after an in-place operation of torch: a backward that saved one of them has to notice."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
@@ -201,6 +206,8 @@ def _paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax
     if plan.counted:
         p.key_weights = key_weights.data_ptr()
     _launch(_capi.load_library().splitd_paged_attn, p, plan.index)
+    if plan.counted:
+        _written(key_weights)
     return out, lse
 
 
@@ -385,6 +392,7 @@ def _paged_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, po
     if cu_seqlens_q is not None:
         p.cu_seqlens = cu_seqlens_q.data_ptr()
     _launch(_capi.load_library().splitd_paged_append, p, plan.index)
+    _written(k_pages, v_pages)
     return q_out
 
 
@@ -531,6 +539,7 @@ def _paged_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_
     p.seqlens_k, p.key_weights = seqlens_k.data_ptr(), key_weights.data_ptr() or _NO_MEMORY
     p.new_seqlens, p.kept, p.new_weights = new_seqlens.data_ptr(), kept.data_ptr(), new_weights.data_ptr()
     _launch(_capi.load_library().splitd_paged_evict, p, plan.index)
+    _written(k_pages, v_pages)
     return new_seqlens, kept, new_weights
 
 

@@ -85,3 +85,59 @@ def test_dispatch_modes_see_the_operators_forward_and_backward():
         y, _ = split_rotary_func(q, None, pos, f)
     assert torch.equal(torch.autograd.grad(y, q, dy)[0], want)
     assert_status_ok()
+
+
+# ---------------------------------------------------------------------------
+# version counters
+# ---------------------------------------------------------------------------
+
+
+def test_writes_raise_the_version_counters():
+    from splitd_flash_attn import split_flash_attn_paged_func, split_paged_append_func, split_paged_evict_func
+
+    q, kk, vv, k, v, table, seqlens, new_table = setup()
+    w = torch.zeros(2, 40, device="cuda")
+
+    def versions():
+        return k._version, v._version, w._version, q._version, kk._version, seqlens._version, table._version
+
+    before = versions()
+    split_paged_append_func(q, kk, vv, k, v, table, seqlens)
+    after = versions()
+    assert after[0] > before[0] and after[1] > before[1] and after[2:] == before[2:]
+    before = after
+    split_flash_attn_paged_func(q, k, v, table, seqlens)
+    assert versions() == before
+    split_flash_attn_paged_func(q, k, v, table, seqlens, key_weights=w)
+    after = versions()
+    assert after[2] > before[2] and after[:2] == before[:2] and after[3:] == before[3:]
+    before = after
+    split_paged_evict_func(k, v, table, seqlens, w, new_table, 24)
+    after = versions()
+    assert after[0] > before[0] and after[1] > before[1] and after[2:] == before[2:]
+    # of the tensor that a view belongs to
+    kv = torch.stack((k, v), 1)
+    before = kv._version
+    split_paged_append_func(q, kk, vv, kv[:, 0], kv[:, 1], table, seqlens)
+    assert kv._version > before
+
+
+def test_autograd_notices_that_a_saved_cache_was_written():
+    from splitd_flash_attn import split_paged_append_func
+
+    q, kk, vv, k, v, table, seqlens, _ = setup()
+    x = torch.ones(1, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    y = (x * k).sum()  # saves k
+    split_paged_append_func(q, kk, vv, k, v, table, seqlens)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_caches_made_in_inference_mode():
+    """They have no version counter."""
+    with torch.inference_mode():
+        args = [*setup(), torch.zeros(2, 40, device="cuda"), freq(512)]
+        want = step(*[a.clone() for a in args])
+        got = step(*args)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert_status_ok()
