@@ -46,6 +46,7 @@ from .rotary import (
     _meta,
     _model,
     _position_strides,
+    _refuse_tangents,
     _rows_fit,
     _token_strides,
     _traced,
@@ -271,6 +272,7 @@ def split_flash_attn_paged_func(
         raise TypeError("window_size must be a tuple of (left, right)")
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
         raise NotImplementedError("SplitD paged attention has no backward: call it under torch.no_grad() or detach its inputs")
+    _refuse_tangents("paged attention", q, k_pages, v_pages, key_weights)
     softmax_scale = _SCALE if softmax_scale is None else float(softmax_scale)
     left, right = (None if w is None else int(w) for w in window_size)
     causal, softcap = bool(causal), float(softcap)
@@ -457,6 +459,7 @@ def split_paged_append_func(
         k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (q is not None and q.requires_grad)
     ):
         raise NotImplementedError("SplitD paged append has no backward: call it under torch.no_grad() or detach its inputs")
+    _refuse_tangents("paged append", q, k, v, k_pages, v_pages, inv_freq)
     interleaved, factor = bool(interleaved), float(factor)
     if _traced(k, k_pages):
         args = (q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q)
@@ -588,6 +591,7 @@ def split_paged_evict_func(
     ``split_paged_append_func``.
     """
     args = (k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
+    _refuse_tangents("paged eviction", k_pages, v_pages, key_weights)
     if _traced(k_pages):
         _check_evict(*args)
         return torch.ops.splitd_flash_attn.paged_evict(*args)

@@ -8,6 +8,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi
 from .interface import SUPPORTED_HEAD_DIM
@@ -133,6 +134,18 @@ def _traced(*tensors) -> bool:
         or bool(torch._C._dispatch_tls_local_include_set().raw_repr() & ~_USUAL_KEYS)
         or any(t is not None and type(t) is not torch.Tensor for t in tensors)
     )
+
+
+def _dual(*tensors) -> bool:
+    """Whether one of them carries a tangent (forward mode). Such a tensor looks like any other."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors
+    )
+
+
+def _refuse_tangents(what: str, *tensors) -> None:
+    if _dual(*tensors):
+        raise NotImplementedError(f"SplitD {what} has no forward-mode derivative: it would be lost without a word")
 
 
 # ---------------------------------------------------------------------------
@@ -265,14 +278,21 @@ def _rotary(q, k, positions, inv_freq, interleaved, factor, backward):
 
 
 class RotaryFunc(torch.autograd.Function):
-    """The map is linear in q and k; its gradient is the same map with the angle's sign turned."""
+    """The map is linear in q and k: a tangent goes through it as they do, and its gradient is the same map with the
+    angle's sign turned."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, interleaved, factor, backward):
         ctx.save_for_backward(positions, inv_freq)
+        ctx.save_for_forward(positions, inv_freq)
         ctx.how = interleaved, factor, backward
         ctx.set_materialize_grads(False)
         return _rotary(q, k, positions, inv_freq, interleaved, factor, backward)
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *none):
+        positions, inv_freq = ctx.saved_tensors
+        return _turned(tq, tk, positions, inv_freq, *ctx.how)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -331,11 +351,18 @@ torch.library.register_autograd("splitd_flash_attn::rotary", _rotary_backward, s
 
 
 def _turned(q, k, positions, inv_freq, interleaved, factor, backward):
+    dual = _dual(q, k)
     if _traced(q, k):
+        if dual:
+            raise NotImplementedError("SplitD rotary positions in forward mode cannot be traced or transformed")
         _check_rotary(q, k, positions, inv_freq)
         q_out, k_out = torch.ops.splitd_flash_attn.rotary(q, k, positions, inv_freq, interleaved, factor, backward)
         return (None if q is None else q_out), (None if k is None else k_out)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
+    if dual and q is not None and k is not None and _dual(q) != _dual(k):  # an output without a tangent is a call of its own
+        _check_rotary(q, k, positions, inv_freq)
+        how = positions, inv_freq, interleaved, factor, backward
+        return _turned(q, None, *how)[0], _turned(None, k, *how)[1]
+    if dual or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
         return RotaryFunc.apply(q, k, positions, inv_freq, interleaved, factor, backward)
     return _rotary(q, k, positions, inv_freq, interleaved, factor, backward)
 
@@ -349,7 +376,7 @@ def split_rotary_func(
     factor: float = 1.0,
 ):
     """Rotary positions on the first ``2 * len(inv_freq)`` dimensions of every head of q and k. Returns
-    ``(q_out, k_out)``, differentiable in q and k.
+    ``(q_out, k_out)``, differentiable in q and k, in forward mode too.
 
     q (B, S, Hq, 512), k (B, S, Hkv, 512), bf16 or fp16, any strides; or packed, (T, Hq, 512) and (T, Hkv, 512). Either
     may be None, and so is its output then. ``positions``: int32 or int64, (B, S), (S,) for all sequences alike, or
@@ -357,4 +384,5 @@ def split_rotary_func(
     far positions lose nothing. A pair is dimensions (i, i + rotary_dim / 2), with ``interleaved`` (2 i, 2 i + 1).
     ``factor`` scales what is rotated; the dimensions behind pass through unchanged.
     """
+    _refuse_tangents("rotary positions with respect to inv_freq", inv_freq)
     return _turned(q, k, positions, inv_freq, bool(interleaved), float(factor), False)

@@ -141,3 +141,114 @@ def test_caches_made_in_inference_mode():
         got = step(*args)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert_status_ok()
+
+
+# ---------------------------------------------------------------------------
+# forward mode
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_tangents_are_rotated(interleaved):
+    """Against the 64-bit form of the tangent's rotation; and against differences: the map is linear."""
+    from torch.autograd import forward_ad
+    from splitd_flash_attn import split_rotary_func
+
+    q, k, tq = (tokens((2, 5), h, torch.float16, s) for h, s in ((4, 1), (2, 2), (4, 3)))
+    pos, f = torch.arange(5, device="cuda") + 1000, freq(256)
+    plain = split_rotary_func(q, k, pos, f, interleaved=interleaved, factor=1.25)
+    ref, tol = rotate_ref(tq, pos.expand(2, 5), f, interleaved, 1.25)
+    for grad in (False, True):
+        x = q.clone().requires_grad_(grad)
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(x, tq)
+            y, z = split_rotary_func(dual, k, pos, f, interleaved=interleaved, factor=1.25)
+            y, t = forward_ad.unpack_dual(y)
+            assert forward_ad.unpack_dual(z).tangent is None
+            assert torch.equal(y, plain[0]) and torch.equal(z, plain[1])
+            assert_within(t, ref, tol, "tangent")
+            assert y.requires_grad == grad
+            y2, z2 = split_rotary_func(q, forward_ad.make_dual(k, k), pos, f, interleaved=interleaved, factor=1.25)
+            assert forward_ad.unpack_dual(y2).tangent is None
+            assert torch.equal(forward_ad.unpack_dual(z2).tangent, plain[1])
+    moved, _ = split_rotary_func(q + tq, None, pos, f, interleaved=interleaved, factor=1.25)
+    # q + tq, both results and their difference are rounded to fp16: half a step of each
+    u = 2.0**-11 * 1.01
+    bound = u * (moved.abs() + plain[0].abs()).double() + tol + 2.0**-24
+    bound += 1.25 * u * 2 * (q + tq).abs().double().amax(-1, keepdim=True)
+    assert ((moved.double() - plain[0].double() - ref).abs() <= bound).all()
+    assert_status_ok()
+
+
+def test_reverse_over_forward():
+    """The tangent is itself differentiable: its gradient is the rotation backwards."""
+    from torch.autograd import forward_ad
+    from splitd_flash_attn import split_rotary_func
+
+    q, dy = tokens((1, 9), 2, torch.bfloat16, 1), tokens((1, 9), 2, torch.bfloat16, 2)
+    tq = tokens((1, 9), 2, torch.bfloat16, 3).requires_grad_()
+    pos, f = torch.arange(9, device="cuda"), freq(512)
+    with forward_ad.dual_level():
+        y, _ = split_rotary_func(forward_ad.make_dual(q, tq), None, pos, f)
+        (g,) = torch.autograd.grad(forward_ad.unpack_dual(y).tangent, tq, dy)
+    x = q.clone().requires_grad_()
+    (want,) = torch.autograd.grad(split_rotary_func(x, None, pos, f)[0], x, dy)
+    assert torch.equal(g, want)
+
+
+def test_tangents_that_would_be_lost_are_refused():
+    from torch.autograd import forward_ad
+    from splitd_flash_attn import split_flash_attn_paged_func, split_paged_append_func, split_paged_evict_func, split_rotary_func
+
+    q, kk, vv, k, v, table, seqlens, new_table = setup()
+    w, f, pos = torch.zeros(2, 40, device="cuda"), freq(512), torch.arange(1, device="cuda")
+    k0 = k.clone()
+    with forward_ad.dual_level():
+        def d(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        calls = (
+            [lambda a=a: split_flash_attn_paged_func(*a, table, seqlens) for a in ((d(q), k, v), (q, d(k), v), (q, k, d(v)))]
+            + [lambda a=a: split_paged_append_func(*a, table, seqlens) for a in (
+                (d(q), kk, vv, k, v), (q, d(kk), vv, k, v), (q, kk, d(vv), k, v), (q, kk, vv, d(k), v), (q, kk, vv, k, d(v)))]
+            + [lambda a=a: split_paged_evict_func(*a[:2], table, seqlens, a[2], new_table, 24) for a in ((d(k), v, w), (k, d(v), w), (k, v, d(w)))]
+            + [lambda: split_flash_attn_paged_func(q, k, v, table, seqlens, key_weights=d(w)),
+               lambda: split_paged_append_func(q, kk, vv, k, v, table, seqlens, inv_freq=d(f)),
+               lambda: split_rotary_func(q, None, pos, d(f))]
+        )
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with Names(), pytest.raises(NotImplementedError, match="forward mode"):
+            split_rotary_func(d(q), None, pos, f)
+        # without a tangent everything goes on as ever
+        out = split_flash_attn_paged_func(q, k, v, table, seqlens)
+        assert torch.equal(split_rotary_func(q, None, pos, f)[0], split_rotary_func(q.clone(), None, pos, f)[0])
+    assert torch.equal(out, split_flash_attn_paged_func(q, k, v, table, seqlens)) and torch.equal(k, k0)
+    assert_status_ok()
+
+
+def test_function_transforms_are_right_or_refused():
+    from splitd_flash_attn import split_rotary_func
+
+    q, dy = tokens((3, 5), 4, torch.bfloat16, 1), tokens((3, 5), 4, torch.bfloat16, 2)
+    pos, f = torch.arange(5, device="cuda"), freq(512)
+    want = split_rotary_func(q, None, pos, f)[0]
+    x = q.clone().requires_grad_()
+    (grad,) = torch.autograd.grad(split_rotary_func(x, None, pos, f)[0], x, dy)
+
+    def fn(x):
+        return split_rotary_func(x, None, pos, f)[0]
+
+    def either(call, value):
+        try:
+            got = call()
+        except (RuntimeError, NotImplementedError):
+            return
+        assert torch.equal(got, value)
+
+    either(lambda: torch.func.functionalize(fn)(q), want)
+    either(lambda: torch.vmap(lambda x: fn(x[None])[0])(q), want)
+    either(lambda: torch.func.vjp(fn, q)[1](dy)[0], grad)
+    either(lambda: torch.func.jvp(fn, (q,), (dy,))[1], split_rotary_func(dy, None, pos, f)[0])
+    assert_status_ok()
