@@ -19,6 +19,7 @@ import os
 from typing import Callable, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _capi
 
@@ -1075,6 +1076,18 @@ torch.library.register_autograd(
 # ---------------------------------------------------------------------------
 
 
+def _dual(*tensors) -> bool:
+    """Whether one of them carries a tangent (forward mode). Such a tensor looks like any other."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors
+    )
+
+
+def _refuse_tangents(what: str, *tensors) -> None:
+    if _dual(*tensors):
+        raise NotImplementedError(f"SplitD {what} has no forward-mode derivative: it would be lost without a word")
+
+
 def _wants_residual(q, k, v) -> bool:
     """A forward whose result can be differentiated keeps the low word of the output (if that is switched on)."""
     return bool(_KEEP_RESIDUAL) and torch.is_grad_enabled() and any(
@@ -1084,8 +1097,10 @@ def _wants_residual(q, k, v) -> bool:
 
 def _reject_unsupported_training(q, k, v, softcap, window_size) -> None:
     """Inside a custom op the tensors no longer say whether they require grad, so what training does not
-    support (fp16, softcap, sliding windows; interface.py:133-138,264-286 of the reference) is refused here."""
+    support (fp16, softcap, sliding windows; interface.py:133-138,264-286 of the reference) is refused here, and so are
+    tangents, which a custom op would drop."""
     tensors = [t for t in (q, k, v) if isinstance(t, torch.Tensor)]
+    _refuse_tangents("attention", *tensors)
     if not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)):
         return
     _validate_training_dtype(q, True)

@@ -30,6 +30,7 @@ from .interface import (
     SUPPORTED_HEAD_DIM,
     _dec,
     _enc,
+    _refuse_tangents,
     _resolve_causal_local_window,
     _status_flag,
     _validate_cu_seqlens,
@@ -46,7 +47,6 @@ from .rotary import (
     _meta,
     _model,
     _position_strides,
-    _refuse_tangents,
     _rows_fit,
     _token_strides,
     _traced,

@@ -8,10 +8,9 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd import forward_ad
 
 from . import _capi
-from .interface import SUPPORTED_HEAD_DIM
+from .interface import SUPPORTED_HEAD_DIM, _dual, _refuse_tangents
 
 __all__ = ["split_rotary_frequencies", "split_rotary_func"]
 
@@ -134,18 +133,6 @@ def _traced(*tensors) -> bool:
         or bool(torch._C._dispatch_tls_local_include_set().raw_repr() & ~_USUAL_KEYS)
         or any(t is not None and type(t) is not torch.Tensor for t in tensors)
     )
-
-
-def _dual(*tensors) -> bool:
-    """Whether one of them carries a tangent (forward mode). Such a tensor looks like any other."""
-    return forward_ad._current_level >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors
-    )
-
-
-def _refuse_tangents(what: str, *tensors) -> None:
-    if _dual(*tensors):
-        raise NotImplementedError(f"SplitD {what} has no forward-mode derivative: it would be lost without a word")
 
 
 # ---------------------------------------------------------------------------
