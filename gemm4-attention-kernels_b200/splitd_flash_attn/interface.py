@@ -1088,6 +1088,12 @@ def _refuse_tangents(what: str, *tensors) -> None:
         raise NotImplementedError(f"SplitD {what} has no forward-mode derivative: it would be lost without a word")
 
 
+def _refuse_derivatives(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError(f"SplitD {what} has no backward: call it under torch.no_grad() or detach its inputs")
+    _refuse_tangents(what, *tensors)
+
+
 def _wants_residual(q, k, v) -> bool:
     """A forward whose result can be differentiated keeps the low word of the output (if that is switched on)."""
     return bool(_KEEP_RESIDUAL) and torch.is_grad_enabled() and any(

@@ -30,7 +30,7 @@ from .interface import (
     SUPPORTED_HEAD_DIM,
     _dec,
     _enc,
-    _refuse_tangents,
+    _refuse_derivatives,
     _resolve_causal_local_window,
     _status_flag,
     _validate_cu_seqlens,
@@ -270,9 +270,7 @@ def split_flash_attn_paged_func(
     """
     if not isinstance(window_size, tuple) or len(window_size) != 2:
         raise TypeError("window_size must be a tuple of (left, right)")
-    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
-        raise NotImplementedError("SplitD paged attention has no backward: call it under torch.no_grad() or detach its inputs")
-    _refuse_tangents("paged attention", q, k_pages, v_pages, key_weights)
+    _refuse_derivatives("paged attention", q, k_pages, v_pages, key_weights)
     softmax_scale = _SCALE if softmax_scale is None else float(softmax_scale)
     left, right = (None if w is None else int(w) for w in window_size)
     causal, softcap = bool(causal), float(softcap)
@@ -455,11 +453,7 @@ def split_paged_append_func(
     Positions are the slots, unless ``positions`` (one per token, int32 or int64) says otherwise, as it has to after an
     eviction.
     """
-    if torch.is_grad_enabled() and (
-        k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad or (q is not None and q.requires_grad)
-    ):
-        raise NotImplementedError("SplitD paged append has no backward: call it under torch.no_grad() or detach its inputs")
-    _refuse_tangents("paged append", q, k, v, k_pages, v_pages, inv_freq)
+    _refuse_derivatives("paged append", q, k, v, k_pages, v_pages, inv_freq)
     interleaved, factor = bool(interleaved), float(factor)
     if _traced(k, k_pages):
         args = (q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, positions, cu_seqlens_q)
@@ -591,7 +585,7 @@ def split_paged_evict_func(
     ``split_paged_append_func``.
     """
     args = (k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
-    _refuse_tangents("paged eviction", k_pages, v_pages, key_weights)
+    _refuse_derivatives("paged eviction", k_pages, v_pages, key_weights)
     if _traced(k_pages):
         _check_evict(*args)
         return torch.ops.splitd_flash_attn.paged_evict(*args)

@@ -10,7 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _capi
-from .interface import SUPPORTED_HEAD_DIM, _dual, _refuse_tangents
+from .interface import SUPPORTED_HEAD_DIM, _dual, _refuse_derivatives
 
 __all__ = ["split_rotary_frequencies", "split_rotary_func"]
 
@@ -367,9 +367,9 @@ def split_rotary_func(
 
     q (B, S, Hq, 512), k (B, S, Hkv, 512), bf16 or fp16, any strides; or packed, (T, Hq, 512) and (T, Hkv, 512). Either
     may be None, and so is its output then. ``positions``: int32 or int64, (B, S), (S,) for all sequences alike, or
-    (T,). ``inv_freq``: float64, radians per position (``split_rotary_frequencies``); angles are formed in 64 bits, so
-    far positions lose nothing. A pair is dimensions (i, i + rotary_dim / 2), with ``interleaved`` (2 i, 2 i + 1).
-    ``factor`` scales what is rotated; the dimensions behind pass through unchanged.
+    (T,). ``inv_freq``: float64, radians per position (``split_rotary_frequencies``), without a gradient; angles are formed
+    in 64 bits, so far positions lose nothing. A pair is dimensions (i, i + rotary_dim / 2), with ``interleaved`` (2 i,
+    2 i + 1). ``factor`` scales what is rotated; the dimensions behind pass through unchanged.
     """
-    _refuse_tangents("rotary positions with respect to inv_freq", inv_freq)
+    _refuse_derivatives("rotary positions with respect to inv_freq", inv_freq)
     return _turned(q, k, positions, inv_freq, bool(interleaved), float(factor), False)
