@@ -53,7 +53,8 @@ struct EvictParams {
   int keep, keep_first, keep_recent;
   int* new_seqlens;   // (batch)
   int* kept;          // (batch, keep), -1 behind the last one
-  float* new_weights; // (batch, keep), 0 behind the last one
+  float* new_weights; // (batch, new_weights_len), 0 behind the last one
+  int new_weights_len;  // >= keep
   int* status;
   int cached;  // keys a CTA has room for in shared memory
 };
@@ -100,6 +101,8 @@ __global__ void __launch_bounds__(kThreads, 1) splitd_evict_select_kernel(const 
   const int m = min(n, p.keep);
   if (gtid == 0 && p.status && stated > n) atomicCAS(p.status, 0, ST_BAD_CACHE_LEN);
   int* kept = p.kept + static_cast<int64_t>(b) * p.keep;
+  // the copy writes the first `keep` of them
+  for (int i = p.keep + gtid; i < p.new_weights_len; i += step) p.new_weights[static_cast<int64_t>(b) * p.new_weights_len + i] = 0.f;
   if (n <= p.keep) {  // the whole cluster: everything stays
     for (int i = gtid; i < p.keep; i += step) kept[i] = i < n ? i : -1;
     if (gtid == 0) p.new_seqlens[b] = m;
@@ -251,7 +254,8 @@ __global__ void __launch_bounds__(kCopyWarps * 32) splitd_evict_copy_kernel(cons
     // whose keys do not fit in shared memory; what is no slot of this cache is not followed.
     int slot = p.kept[at];
     if (slot >= min(page_capacity(p.from), p.weights_len)) slot = -1;
-    if (h == 0 && !is_v) p.new_weights[at] = slot < 0 ? 0.f : __ldg(p.weights + b * p.weights_stride + slot);
+    if (h == 0 && !is_v)
+      p.new_weights[static_cast<int64_t>(b) * p.new_weights_len + place] = slot < 0 ? 0.f : __ldg(p.weights + b * p.weights_stride + slot);
     if (slot >= 0) {
       int entry, in_page;
       split_slot(p.from, slot, entry, in_page);
@@ -321,6 +325,7 @@ int launch_evict(const splitd_evict_params* a, cudaStream_t stream) {
   p.weights = a->key_weights, p.weights_stride = a->key_weights_stride, p.weights_len = a->key_weights_len;
   p.keep = a->keep, p.keep_first = a->keep_first, p.keep_recent = a->keep_recent;
   p.new_seqlens = a->new_seqlens, p.kept = a->kept, p.new_weights = a->new_weights;
+  p.new_weights_len = a->new_weights_len > 0 ? a->new_weights_len : a->keep;
   p.status = a->status_flag;
   int64_t slots = static_cast<int64_t>(a->max_pages) * a->page_size;
   if (a->key_weights_len < slots) slots = a->key_weights_len;

@@ -168,7 +168,7 @@ class SplitdEvictParams(ctypes.Structure):
         """
         ptr: k_pages v_pages page_table new_page_table seqlens_k key_weights new_seqlens kept new_weights status_flag
         i32: batch heads_kv head_dim num_pages page_size max_pages new_max_pages
-        i32: key_weights_len keep keep_first keep_recent
+        i32: key_weights_len keep keep_first keep_recent new_weights_len
         i64: page_table_stride new_page_table_stride key_weights_stride k_strides*3 v_strides*3
         """
     )

@@ -470,13 +470,16 @@ def split_paged_append_func(
 # ---------------------------------------------------------------------------
 
 
-def _check_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent) -> None:
+def _check_evict(
+    k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent, weights_len
+) -> None:
     _check_cache(k_pages, v_pages, page_table, seqlens_k)
     _check_written(k_pages, v_pages)
     batch = seqlens_k.shape[0]
     _check_weights(key_weights, batch, k_pages.device)
     _check_table(new_page_table, "new_page_table", batch, k_pages.device)
-    for name, n in (("keep", keep), ("keep_first", keep_first), ("keep_recent", keep_recent)):
+    counts = ("keep", keep), ("keep_first", keep_first), ("keep_recent", keep_recent), ("weights_len", weights_len)
+    for name, n in counts if weights_len is not None else counts[:3]:
         if isinstance(n, bool) or not isinstance(n, (int, torch.SymInt)):
             raise TypeError(f"{name} must be an int, got {type(n).__name__}")
         if n < 0:
@@ -485,6 +488,8 @@ def _check_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_
         raise ValueError(f"keep ({keep}) must be at least 1 and at least keep_first + keep_recent ({keep_first} + {keep_recent})")
     if keep > 2**30:
         raise ValueError(f"keep ({keep}) must be at most 2^30")
+    if weights_len is not None and not keep <= weights_len < 2**31:
+        raise ValueError(f"weights_len ({weights_len}) must be at least keep ({keep}) and below 2^31")
     if new_page_table.shape[1] * k_pages.shape[1] < keep:
         raise ValueError(
             f"new_page_table has {new_page_table.shape[1]} pages of {k_pages.shape[1]} slots per sequence, too few for {keep}"
@@ -492,20 +497,25 @@ def _check_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_
 
 
 class _EvictPlan:
-    def __init__(self, k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent):
-        _check_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
+    def __init__(
+        self, k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent, weights_len
+    ):
+        _check_evict(
+            k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent, weights_len
+        )
         device, batch = k_pages.device, seqlens_k.shape[0]
         self.index = k_pages.get_device()
         self.fits = _unit_rows(page_table, new_page_table, seqlens_k)
         self.empty = batch == 0
         self.seqlens_model = _model((batch,), torch.int32, device)
         self.kept_model = _model((batch, keep), torch.int32, device)
-        self.weights_model = _model((batch, keep), torch.float32, device)
+        self.weights_model = _model((batch, keep if weights_len is None else weights_len), torch.float32, device)
         p = _capi.SplitdEvictParams()
         _fill_cache(p, k_pages, page_table, device)
         p.new_max_pages, p.new_page_table_stride = new_page_table.shape[1], new_page_table.stride(0)
         p.key_weights_len, p.key_weights_stride = key_weights.shape[1], key_weights.stride(0)
         p.keep, p.keep_first, p.keep_recent = keep, keep_first, keep_recent
+        p.new_weights_len = 0 if weights_len is None else weights_len
         p.k_strides, p.v_strides = k_pages.stride()[:3], v_pages.stride()[:3]
         self.params = bytes(p)
 
@@ -513,11 +523,13 @@ class _EvictPlan:
 _evict_plans = _Plans()
 
 
-def _paged_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent):
-    how = keep, keep_first, keep_recent
+def _paged_evict(
+    k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent, weights_len
+):
+    how = keep, keep_first, keep_recent, weights_len
     key = (
         _meta(k_pages), _meta(v_pages), _meta(page_table), _meta(seqlens_k), _meta(key_weights), _meta(new_page_table), how,
-        type(keep), type(keep_first), type(keep_recent),
+        type(keep), type(keep_first), type(keep_recent), type(weights_len),
     )
     plan = _evict_plans.get(key)
     if plan is None:
@@ -551,15 +563,23 @@ def _paged_evict_custom(
     keep: int,
     keep_first: int,
     keep_recent: int,
+    weights_len: Optional[int] = None,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    return _paged_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
+    return _paged_evict(
+        k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent, weights_len
+    )
 
 
 @torch.library.register_fake("splitd_flash_attn::paged_evict")
-def _paged_evict_fake(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent):
-    _check_evict(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
+def _paged_evict_fake(
+    k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent, weights_len=None
+):
+    _check_evict(
+        k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent, weights_len
+    )
     batch = seqlens_k.shape[0]
-    return seqlens_k.new_empty((batch,)), seqlens_k.new_empty((batch, keep)), key_weights.new_empty((batch, keep))
+    width = keep if weights_len is None else weights_len
+    return seqlens_k.new_empty((batch,)), seqlens_k.new_empty((batch, keep)), key_weights.new_empty((batch, width))
 
 
 def split_paged_evict_func(
@@ -572,6 +592,7 @@ def split_paged_evict_func(
     keep: int,
     keep_first: int = 0,
     keep_recent: int = 0,
+    weights_len: Optional[int] = None,
 ):
     """Shortens every sequence to at most ``keep`` slots: its first ``keep_first``, its last ``keep_recent``, and of the
     others those with the largest ``key_weights`` (of equal ones the lower slot; NaN counts as the largest). The kept keys
@@ -579,12 +600,16 @@ def split_paged_evict_func(
     sequence may be using: pages are often shared between sequences, so none is changed in place. Sequences that are
     short enough already are copied as they are; leave them out of the call to leave them alone.
 
+    ``key_weights`` (B, slots) has to reach as far as the sequences do: one that is longer is cut to it first, which
+    loses its last slots, ``keep_recent`` or not (status 108).
+
     Returns ``(new_seqlens, kept, new_weights)``: (B,) int32 lengths; (B, keep) int32 old slots, ascending, -1 behind
-    the last; (B, keep) float32 their weights, 0 behind the last, which go on being ``key_weights`` of the new cache.
-    Keys keep the rotation of the position they had, so tokens that follow need ``positions`` in
-    ``split_paged_append_func``.
+    the last; (B, weights_len) float32 their weights, 0 behind the last. ``weights_len`` is ``keep`` if not given. To go
+    on with them as ``key_weights`` of the new cache, ask for as many as that may grow to: slots behind the end of
+    ``key_weights`` are not counted. Keys keep the rotation of the position they had, so tokens that follow need
+    ``positions`` in ``split_paged_append_func``.
     """
-    args = (k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent)
+    args = (k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, keep, keep_first, keep_recent, weights_len)
     _refuse_derivatives("paged eviction", k_pages, v_pages, key_weights)
     if _traced(k_pages):
         _check_evict(*args)

@@ -313,8 +313,9 @@ int splitd_paged_append(const splitd_append_params* p, void* stream);
 /* Eviction: of the n = seqlens_k[b] slots of a sequence keep min(n, keep), the first keep_first, the last keep_recent
  * and of the others those with the largest key_weights (equal weights: the lower slot; NaN counts as the largest), and
  * copy their keys and values, in slot order, to the pages of new_page_table, which no sequence of the call may be
- * using. kept[b] gets the old slots (-1 behind the last), new_weights[b] their weights (0 behind the last),
- * new_seqlens[b] their number. A sequence longer than key_weights_len is cut to it (status 108). */
+ * using. kept[b] gets the old slots (-1 behind the last), new_weights[b] their weights (0 behind the last, up to
+ * new_weights_len: what the new cache may grow to, so that they can be its key_weights), new_seqlens[b] their number. A
+ * sequence longer than key_weights_len is cut to it, which loses its last slots (status 108). */
 typedef struct {
   void* k_pages;
   void* v_pages;
@@ -324,11 +325,12 @@ typedef struct {
   const float* key_weights; /* (B, key_weights_len) */
   int32_t* new_seqlens;     /* (B) */
   int32_t* kept;            /* (B, keep) contiguous */
-  float* new_weights;       /* (B, keep) contiguous */
+  float* new_weights;       /* (B, new_weights_len) contiguous */
   int32_t* status_flag;
   int32_t batch, heads_kv, head_dim;
   int32_t num_pages, page_size, max_pages, new_max_pages;
   int32_t key_weights_len, keep, keep_first, keep_recent;
+  int32_t new_weights_len;  /* at least keep; 0: keep */
   int64_t page_table_stride, new_page_table_stride, key_weights_stride;
   int64_t k_strides[3], v_strides[3]; /* page, row of the page, head */
 } splitd_evict_params;
