@@ -313,7 +313,8 @@ def kernel_status(device: Optional[torch.device] = None) -> int:
     The kernels never spin forever: a wait that exceeds 4 s is given up, the kernel ends early and stores a
     code here (101 loads, 102 tensor-core issue, 103 softmax/epilogue, 104 peer CTA, 105 shared-memory
     alignment, 106 a packed sequence longer than max_seqlen_k, 107 a page table that names a page its cache does not
-    have, 108 a sequence longer than its row of the page table). Outputs of such a call are incomplete. The calls
+    have, 108 a sequence longer than its row of the page table or than its key_weights). Outputs of such a call are
+    incomplete, after 107 and 108 as far as the page or the slots behind the end go. The calls
     of this module are asynchronous, so nothing can raise at the call itself: check this after a step (it costs
     one 4-byte copy), e.g. where the loss is read. The packed API looks at it whenever it validates cu_seqlens.
     ``reset_kernel_status()`` re-arms it.
@@ -333,9 +334,13 @@ def _raise_if_a_kernel_gave_up(device: torch.device) -> None:
     if flag is not None:
         code = int(flag.item())
         if code != 0:
+            what = {
+                106: "met a packed sequence longer than max_seqlen_k; its outputs are incomplete",
+                107: "met a page table that names a page its cache does not have; that page was neither read nor written",
+                108: "met a sequence longer than its row of the page table, or than its key_weights, and cut it to that",
+            }.get(code, "ended early; its outputs are incomplete")
             raise RuntimeError(
-                f"an earlier SplitD attention kernel on {device} ended early with status {code} "
-                "(see kernel_status); its outputs are incomplete"
+                f"an earlier SplitD kernel on {device} {what} (status {code}; reset_kernel_status() re-arms it)"
             )
 
 
