@@ -317,7 +317,8 @@ def kernel_status(device: Optional[torch.device] = None) -> int:
     incomplete, after 107 and 108 as far as the page or the slots behind the end go. The calls
     of this module are asynchronous, so nothing can raise at the call itself: check this after a step (it costs
     one 4-byte copy), e.g. where the loss is read. The packed API looks at it whenever it validates cu_seqlens.
-    ``reset_kernel_status()`` re-arms it.
+    ``reset_kernel_status()`` re-arms it. The first call of the library on a device makes the word: where that call is
+    captured in a CUDA graph, every replay zeroes it; make one call before the capture, as torch's warm-up does.
     """
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
     return int(_status_flag(device).item())

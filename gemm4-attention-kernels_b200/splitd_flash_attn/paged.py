@@ -105,9 +105,8 @@ def _page_pointers(k_pages, v_pages):
 _NO_MEMORY = 256
 
 
-def _fill_cache(p, k_pages, page_table, device) -> None:
+def _fill_cache(p, k_pages, page_table) -> None:
     """What the parameter structs have in common."""
-    p.status_flag = _status_flag(device).data_ptr()
     p.batch = page_table.shape[0]
     p.heads_kv, p.head_dim = k_pages.shape[2], SUPPORTED_HEAD_DIM
     p.num_pages, p.page_size = k_pages.shape[:2]
@@ -163,7 +162,7 @@ class _PagedAttnPlan:
         self.out_model = _model(q.shape, q.dtype, q.device)
         self.lse_model = _model((batch, hq, sq), torch.float32, q.device)
         p = _capi.SplitdPagedParams()
-        _fill_cache(p, k_pages, page_table, q.device)
+        _fill_cache(p, k_pages, page_table)
         p.seqlen_q, p.heads_q, p.dtype = sq, hq, _DTYPES[q.dtype]
         p.causal, p.local = int(causal), int(local)
         p.window_left = -1 if left is None or left < 0 else min(left, 2**31 - 1)
@@ -199,6 +198,7 @@ def _paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax
         return out, lse
     workspace = torch.empty_like(plan.workspace_model)
     p = _capi.SplitdPagedParams.from_buffer_copy(plan.params)
+    p.status_flag = _status_flag(q.device).data_ptr()
     p.q, p.o, p.workspace = q_at, out.data_ptr(), workspace.data_ptr()
     p.k_pages, p.v_pages = _page_pointers(k_pages, v_pages)
     p.page_table, p.seqlens_k = page_table.data_ptr() or _NO_MEMORY, seqlens_k.data_ptr()
@@ -339,7 +339,7 @@ class _AppendPlan:
         self.empty = k.numel() == 0
         self.q_model = None if q is None else _model(q.shape, q.dtype, q.device)
         p = _capi.SplitdAppendParams()
-        _fill_cache(p, k_pages, page_table, k.device)
+        _fill_cache(p, k_pages, page_table)
         p.seqlen, p.total_tokens = (0, k.shape[0]) if packed else (k.shape[1], 0)
         p.dtype, p.rotary_dim, p.interleaved, p.factor = _DTYPES[k.dtype], 2 * self.pairs, int(interleaved), factor
         if positions is not None:
@@ -378,6 +378,7 @@ def _paged_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, po
     if plan.empty:
         return q_out
     p = _capi.SplitdAppendParams.from_buffer_copy(plan.params)
+    p.status_flag = _status_flag(k.device).data_ptr()
     p.k, p.v = k_at, v_at
     p.k_pages, p.v_pages = _page_pointers(k_pages, v_pages)
     if p.k_pages == p.v_pages and k_pages.numel():
@@ -511,7 +512,7 @@ class _EvictPlan:
         self.kept_model = _model((batch, keep), torch.int32, device)
         self.weights_model = _model((batch, keep if weights_len is None else weights_len), torch.float32, device)
         p = _capi.SplitdEvictParams()
-        _fill_cache(p, k_pages, page_table, device)
+        _fill_cache(p, k_pages, page_table)
         p.new_max_pages, p.new_page_table_stride = new_page_table.shape[1], new_page_table.stride(0)
         p.key_weights_len, p.key_weights_stride = key_weights.shape[1], key_weights.stride(0)
         p.keep, p.keep_first, p.keep_recent = keep, keep_first, keep_recent
@@ -543,6 +544,7 @@ def _paged_evict(
     if plan.empty:
         return new_seqlens, kept, new_weights
     p = _capi.SplitdEvictParams.from_buffer_copy(plan.params)
+    p.status_flag = _status_flag(k_pages.device).data_ptr()
     p.k_pages, p.v_pages = _page_pointers(k_pages, v_pages)
     p.page_table, p.new_page_table = page_table.data_ptr() or _NO_MEMORY, new_page_table.data_ptr()
     p.seqlens_k, p.key_weights = seqlens_k.data_ptr(), key_weights.data_ptr() or _NO_MEMORY
