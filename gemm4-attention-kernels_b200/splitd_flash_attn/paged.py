@@ -184,7 +184,7 @@ _paged_attn_plans = _Plans()
 def _paged_attn(q, k_pages, v_pages, page_table, seqlens_k, key_weights, softmax_scale, causal, left, right, softcap, want_lse):
     how = softmax_scale, causal, left, right, softcap
     key = (_meta(q), _meta(k_pages), _meta(v_pages), _meta(page_table), _meta(seqlens_k), _meta(key_weights), how)
-    plan = _paged_attn_plans.get(key)
+    plan = _paged_attn_plans.find(key)
     if plan is None:
         plan = _paged_attn_plans.keep(key, _PagedAttnPlan(q, k_pages, v_pages, page_table, seqlens_k, key_weights, *how))
     q_at = q.data_ptr()
@@ -359,7 +359,7 @@ def _paged_append(q, k, v, k_pages, v_pages, page_table, seqlens_k, inv_freq, po
         _meta(q), _meta(k), _meta(v), _meta(k_pages), _meta(v_pages), _meta(page_table), _meta(seqlens_k), _meta(inv_freq),
         _meta(positions), _meta(cu_seqlens_q), interleaved, factor,
     )
-    plan = _append_plans.get(key)
+    plan = _append_plans.find(key)
     if plan is None:
         plan = _append_plans.keep(
             key,
@@ -532,7 +532,7 @@ def _paged_evict(
         _meta(k_pages), _meta(v_pages), _meta(page_table), _meta(seqlens_k), _meta(key_weights), _meta(new_page_table), how,
         type(keep), type(keep_first), type(keep_recent), type(weights_len),
     )
-    plan = _evict_plans.get(key)
+    plan = _evict_plans.find(key)
     if plan is None:
         plan = _evict_plans.keep(key, _EvictPlan(k_pages, v_pages, page_table, seqlens_k, key_weights, new_page_table, *how))
     if not plan.fits:

@@ -10,7 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _capi
-from .interface import SUPPORTED_HEAD_DIM, _dual, _refuse_derivatives
+from .interface import SUPPORTED_HEAD_DIM, _dual, _refuse_derivatives, _status_flag
 
 __all__ = ["split_rotary_frequencies", "split_rotary_func"]
 
@@ -141,15 +141,26 @@ def _traced(*tensors) -> bool:
 # A decode step's kernels take a few microseconds, less than checking a dozen tensors, filling a parameter struct and
 # allocating in Python do. So what a call's shapes, strides, types and options decide is worked out once and kept under
 # exactly those: that the arguments are fine, the filled struct (as bytes; each call puts its pointers into a copy) and
-# models of the outputs. No pointer to and no value of a caller's tensor is part of it.
+# models of the outputs. No pointer to and no value of a caller's tensor is part of it, and no device memory. Of more than
+# _PLANS_MOST, the one that was not used for the longest time goes: packed prompts bring a new number of tokens with nearly
+# every call, and must not push out the decode steps' plans.
 
 _PLANS_MOST = 1024
 
 
 class _Plans(dict):
+    """In the order of their last use. A plan that two threads look for at once may be made twice."""
+
+    def find(self, key):
+        plan = self.pop(key, None)
+        if plan is not None:
+            self[key] = plan
+        return plan
+
     def keep(self, key, plan):
-        if len(self) >= _PLANS_MOST:
-            self.clear()
+        while len(self) >= _PLANS_MOST:
+            for oldest in list(self)[:1]:
+                self.pop(oldest, None)
         self[key] = plan
         return plan
 
@@ -159,8 +170,9 @@ def _meta(t: Optional[torch.Tensor]):
 
 
 def _model(shape, dtype, device) -> torch.Tensor:
-    """``empty_like`` of it is a contiguous tensor of that shape and costs half of ``empty``; it has one element itself."""
-    return torch.empty((), dtype=dtype, device=device).expand(shape)
+    """``empty_like`` of it is a contiguous tensor of that shape and costs half of ``empty``; its one element is the status
+    word's memory, which is there anyway."""
+    return _status_flag(device).view(dtype)[0].expand(shape)
 
 
 def _rows_fit(t: Optional[torch.Tensor]) -> bool:
@@ -237,7 +249,7 @@ _rotary_plans = _Plans()
 def _rotary(q, k, positions, inv_freq, interleaved, factor, backward):
     """One launch for both; None stays None."""
     key = (_meta(q), _meta(k), _meta(positions), _meta(inv_freq), interleaved, factor, backward)
-    plan = _rotary_plans.get(key)
+    plan = _rotary_plans.find(key)
     if plan is None:
         plan = _rotary_plans.keep(key, _RotaryPlan(q, k, positions, inv_freq, interleaved, factor, backward))
     q_at = q.data_ptr() if plan.has_q else 0

@@ -54,3 +54,36 @@ def test_the_status_word_of_now_is_used(fresh_status):
         assert kernel_status() == 107
         assert all(int(f) == 0 for f in before.values())
         reset_kernel_status()
+
+
+def test_plans_hold_no_device_memory():
+    """Prompts of ever new lengths leave nothing on the device, in a capture neither."""
+    from splitd_flash_attn import split_flash_attn_paged_func, split_paged_append_func, split_rotary_func
+    from splitd_flash_attn.interface import cu_seqlens_validation
+
+    k, v, table, _, seqlens, _ = cache()
+    pos, f = torch.zeros(1000, dtype=torch.int32, device="cuda"), freq(64)
+    q = tokens((1000,), 2, torch.bfloat16, 2)
+    cu = torch.zeros(3, dtype=torch.int32, device="cuda")
+
+    def calls(n):
+        split_rotary_func(q[:n], q[:n, :1], pos[:n], f)
+        with cu_seqlens_validation(False):
+            split_paged_append_func(q[:n], q[:n, :1], q[:n, :1], k, v, table, seqlens, cu_seqlens_q=cu)
+        split_flash_attn_paged_func(q[:2, None], k, v, table.repeat(1, 1 + n), seqlens)
+
+    calls(999)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for n in range(1, 60):
+        calls(n)
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(100)
+    graph.replay()
+    torch.cuda.synchronize()
+    del graph
+    assert torch.cuda.memory_allocated() == before
+    assert_status_ok()
