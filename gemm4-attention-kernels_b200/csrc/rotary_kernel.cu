@@ -250,7 +250,7 @@ namespace {
 
 template <bool kFp16, int kLayout>
 void launch_layout(const RotaryParams& p, unsigned blocks, cudaStream_t stream) {
-  if (blocks <= 2 * 148)
+  if (blocks <= 2u * sm_count())
     rot::splitd_rotary_kernel<kFp16, kLayout, 2><<<blocks, rot::kWarps * 32, 0, stream>>>(p);
   else
     rot::splitd_rotary_kernel<kFp16, kLayout, 3><<<blocks, rot::kWarps * 32, 0, stream>>>(p);
@@ -269,16 +269,17 @@ int launch_rotary_kernel(RotaryParams& p, bool fp16, bool interleaved, cudaStrea
   // much as five of its heads, and much longer runs leave a tail (37 x 46 tokens, 40 heads: 25 us with two runs, 33 us with
   // three of 14, 34 us with ten of 4; 2 x 8192 tokens, 36 heads: 193 us with three runs, 201 us with two of 18). Shorter
   // runs when there would not be half as many warps as the GPU holds (6 x 103 tokens, 36 heads: 11 us with three runs, 13
-  // us with two), but four heads, one round of loads, at least. Calls of up to one wave of blocks get the registers of two blocks per SM (64 tokens: 5.7 us, 6.5 us
-  // with three), longer ones three blocks (2 x 8192 tokens: 195 us, 201 us with two).
-  constexpr int64_t kHalfFull = 148 * 24 / 2;
+  // us with two), but four heads, one round of loads, at least. Calls of up to one wave of blocks get the registers of two
+  // blocks per SM (64 tokens: 5.7 us, 6.5 us with three), longer ones three blocks (2 x 8192 tokens: 195 us, 201 us with
+  // two).
+  const int64_t half_full = sm_count() * (3 * rot::kWarps) / 2;
   int64_t groups = (heads + 19) / 20;
   for (int64_t g = groups; g <= 2 * groups; ++g)
     if (heads % (4 * g) == 0) {
       groups = g;
       break;
     }
-  const int64_t fill = (kHalfFull + p.tokens - 1) / p.tokens, most = (heads + rot::kUnroll - 1) / rot::kUnroll;
+  const int64_t fill = (half_full + p.tokens - 1) / p.tokens, most = (heads + rot::kUnroll - 1) / rot::kUnroll;
   if (groups < fill) groups = fill < most ? fill : most;
   p.heads_per_warp = static_cast<int>((heads + groups - 1) / groups);
   p.groups = (heads + p.heads_per_warp - 1) / p.heads_per_warp;
