@@ -1095,9 +1095,12 @@ def _refuse_tangents(what: str, *tensors) -> None:
 
 
 def _refuse_derivatives(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise NotImplementedError(f"SplitD {what} has no backward: call it under torch.no_grad() or detach its inputs")
-    _refuse_tangents(what, *tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise NotImplementedError(f"SplitD {what} has no backward: call it under torch.no_grad() or detach its inputs")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(what, *tensors)
 
 
 def _wants_residual(q, k, v) -> bool:

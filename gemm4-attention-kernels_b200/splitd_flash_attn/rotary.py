@@ -4,6 +4,7 @@ call it). Kernel: ``csrc/rotary_kernel.cu``; C-ABI: ``splitd_rotary``."""
 from __future__ import annotations
 
 import ctypes
+import itertools
 import math
 from typing import Optional, Tuple
 
@@ -119,7 +120,7 @@ def _token_strides(t: torch.Tensor):
 
 
 # Dispatch keys that every thread includes; any other belongs to something that wants to see each operator.
-_USUAL_KEYS = (
+_UNUSUAL_KEYS = ~(
     torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect) | torch._C.DispatchKeySet(torch._C.DispatchKey.ADInplaceOrView)
 ).raw_repr()
 
@@ -128,11 +129,12 @@ def _traced(*tensors) -> bool:
     """Whether the call goes through its custom op: under torch.compile, for tensors without memory and other subclasses, and
     where a tracer, a dispatch mode or a function transform is at work. Otherwise the kernel is called without the
     dispatcher, which costs several times what the kernels of a decode step take."""
-    return (
-        torch.compiler.is_compiling()
-        or bool(torch._C._dispatch_tls_local_include_set().raw_repr() & ~_USUAL_KEYS)
-        or any(t is not None and type(t) is not torch.Tensor for t in tensors)
-    )
+    if torch.compiler.is_compiling() or torch._C._dispatch_tls_local_include_set().raw_repr() & _UNUSUAL_KEYS:
+        return True
+    for t in tensors:
+        if t is not None and type(t) is not torch.Tensor:
+            return True
+    return False
 
 
 # ---------------------------------------------------------------------------
@@ -149,19 +151,24 @@ _PLANS_MOST = 1024
 
 
 class _Plans(dict):
-    """In the order of their last use. A plan that two threads look for at once may be made twice."""
+    """[plan, time of its last use] under its key. Two threads that look for a plan at once may both make it."""
+
+    def __init__(self):
+        super().__init__()
+        self.clock = itertools.count()
 
     def find(self, key):
-        plan = self.pop(key, None)
-        if plan is not None:
-            self[key] = plan
-        return plan
+        entry = self.get(key)
+        if entry is None:
+            return None
+        entry[1] = next(self.clock)
+        return entry[0]
 
     def keep(self, key, plan):
-        while len(self) >= _PLANS_MOST:
-            for oldest in list(self)[:1]:
-                self.pop(oldest, None)
-        self[key] = plan
+        if len(self) >= _PLANS_MOST:
+            oldest = min(list(self.items()), key=lambda item: item[1][1])
+            self.pop(oldest[0], None)
+        self[key] = [plan, next(self.clock)]
         return plan
 
 
@@ -277,21 +284,14 @@ def _rotary(q, k, positions, inv_freq, interleaved, factor, backward):
 
 
 class RotaryFunc(torch.autograd.Function):
-    """The map is linear in q and k: a tangent goes through it as they do, and its gradient is the same map with the
-    angle's sign turned."""
+    """The map is linear in q and k; its gradient is the same map with the angle's sign turned."""
 
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, interleaved, factor, backward):
         ctx.save_for_backward(positions, inv_freq)
-        ctx.save_for_forward(positions, inv_freq)
         ctx.how = interleaved, factor, backward
         ctx.set_materialize_grads(False)
         return _rotary(q, k, positions, inv_freq, interleaved, factor, backward)
-
-    @staticmethod
-    def jvp(ctx, tq, tk, *none):
-        positions, inv_freq = ctx.saved_tensors
-        return _turned(tq, tk, positions, inv_freq, *ctx.how)
 
     @staticmethod
     def backward(ctx, dq, dk):
@@ -305,6 +305,20 @@ class RotaryFunc(torch.autograd.Function):
             return (None,) * 7
         dq, dk = _turned(dq, dk, positions, inv_freq, interleaved, factor, not backward)
         return dq, dk, None, None, None, None, None
+
+
+class RotaryDualFunc(RotaryFunc):
+    """Of inputs that carry tangents, which go through the map as they do."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, inv_freq, interleaved, factor, backward):
+        ctx.save_for_forward(positions, inv_freq)
+        return RotaryFunc.forward(ctx, q, k, positions, inv_freq, interleaved, factor, backward)
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *none):
+        positions, inv_freq = ctx.saved_tensors
+        return _turned(tq, tk, positions, inv_freq, *ctx.how)
 
 
 @torch.library.custom_op("splitd_flash_attn::rotary", mutates_args=())
@@ -350,20 +364,24 @@ torch.library.register_autograd("splitd_flash_attn::rotary", _rotary_backward, s
 
 
 def _turned(q, k, positions, inv_freq, interleaved, factor, backward):
-    dual = _dual(q, k)
+    if _dual(q, k):
+        return _turned_with_tangents(q, k, positions, inv_freq, interleaved, factor, backward)
     if _traced(q, k):
-        if dual:
-            raise NotImplementedError("SplitD rotary positions in forward mode cannot be traced or transformed")
         _check_rotary(q, k, positions, inv_freq)
         q_out, k_out = torch.ops.splitd_flash_attn.rotary(q, k, positions, inv_freq, interleaved, factor, backward)
         return (None if q is None else q_out), (None if k is None else k_out)
-    if dual and q is not None and k is not None and _dual(q) != _dual(k):  # an output without a tangent is a call of its own
-        _check_rotary(q, k, positions, inv_freq)
-        how = positions, inv_freq, interleaved, factor, backward
-        return _turned(q, None, *how)[0], _turned(None, k, *how)[1]
-    if dual or torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k)):
+    if torch.is_grad_enabled() and (q is not None and q.requires_grad or k is not None and k.requires_grad):
         return RotaryFunc.apply(q, k, positions, inv_freq, interleaved, factor, backward)
     return _rotary(q, k, positions, inv_freq, interleaved, factor, backward)
+
+
+def _turned_with_tangents(q, k, *how):
+    if _traced(q, k):
+        raise NotImplementedError("SplitD rotary positions in forward mode cannot be traced or transformed")
+    if q is not None and k is not None and _dual(q) != _dual(k):  # an output without a tangent is a call of its own
+        _check_rotary(q, k, *how[:2])
+        return _turned(q, None, *how)[0], _turned(None, k, *how)[1]
+    return RotaryDualFunc.apply(q, k, *how)
 
 
 def split_rotary_func(
