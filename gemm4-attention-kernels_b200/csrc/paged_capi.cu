@@ -145,8 +145,9 @@ int splitd_paged_evict(const splitd_evict_params* p, void* stream) {
   if (p->new_max_pages < 0 || static_cast<int64_t>(p->new_max_pages) * p->page_size < p->keep)
     return fail(SPLITD_ERR_INVALID_ARGUMENT, "new_page_table: %d pages of %d slots do not hold %d", p->new_max_pages, p->page_size,
                 p->keep);
-  if (p->new_weights_len != 0 && p->new_weights_len < p->keep)
-    return fail(SPLITD_ERR_INVALID_ARGUMENT, "new_weights_len (%d) must be 0 or at least keep (%d)", p->new_weights_len, p->keep);
+  if (p->new_weights_len != 0 && (p->new_weights_len < p->keep || p->new_weights_len > 1 << 30))
+    return fail(SPLITD_ERR_INVALID_ARGUMENT, "new_weights_len (%d) must be 0, or at least keep (%d) and at most 2^30",
+                p->new_weights_len, p->keep);
   if (p->key_weights_len < 0) return fail(SPLITD_ERR_INVALID_ARGUMENT, "key_weights_len must not be negative");
   if (int e = check_rows(p->k_pages, p->k_strides, 0, "k_pages")) return e;
   if (int e = check_rows(p->v_pages, p->v_strides, 0, "v_pages")) return e;

@@ -489,8 +489,8 @@ def _check_evict(
         raise ValueError(f"keep ({keep}) must be at least 1 and at least keep_first + keep_recent ({keep_first} + {keep_recent})")
     if keep > 2**30:
         raise ValueError(f"keep ({keep}) must be at most 2^30")
-    if weights_len is not None and not keep <= weights_len < 2**31:
-        raise ValueError(f"weights_len ({weights_len}) must be at least keep ({keep}) and below 2^31")
+    if weights_len is not None and not keep <= weights_len <= 2**30:
+        raise ValueError(f"weights_len ({weights_len}) must be at least keep ({keep}) and at most 2^30")
     if new_page_table.shape[1] * k_pages.shape[1] < keep:
         raise ValueError(
             f"new_page_table has {new_page_table.shape[1]} pages of {k_pages.shape[1]} slots per sequence, too few for {keep}"

@@ -330,7 +330,7 @@ typedef struct {
   int32_t batch, heads_kv, head_dim;
   int32_t num_pages, page_size, max_pages, new_max_pages;
   int32_t key_weights_len, keep, keep_first, keep_recent;
-  int32_t new_weights_len;  /* at least keep; 0: keep */
+  int32_t new_weights_len;  /* at least keep, at most 2^30; 0: keep */
   int64_t page_table_stride, new_page_table_stride, key_weights_stride;
   int64_t k_strides[3], v_strides[3]; /* page, row of the page, head */
 } splitd_evict_params;

@@ -18,7 +18,7 @@ def test_width_of_the_new_weights(fake):  # noqa: F811
         a, b, c = fn(k, v, t, n, w, new, 32, 2, 3, weights_len=width)
         assert a.shape == (3,) and b.shape == (3, 32) and c.shape == (3, width) and c.dtype == torch.float32
     assert fn(k, v, t, n, w, new, 32, 2, 3, weights_len=None)[2].shape == (3, 32)
-    for width in (31, 0, -1, 2**31):
+    for width in (31, 0, -1, 2**30 + 1, 2**31 - 1, 2**31):
         with pytest.raises(ValueError, match="weights_len"):
             fn(k, v, t, n, w, new, 32, weights_len=width)
     for width in (40.0, True, "40"):
@@ -28,7 +28,7 @@ def test_width_of_the_new_weights(fake):  # noqa: F811
 
 def test_entry_point_refuses_a_narrow_one():
     fn = _capi.load_library().splitd_paged_evict
-    for width in (31, -1):
+    for width in (31, -1, 2**30 + 1, 2**31 - 1):
         p = _capi.SplitdEvictParams()
         for n in ("k_pages", "v_pages", "page_table", "new_page_table", "seqlens_k", "key_weights", "new_seqlens", "kept", "new_weights"):
             setattr(p, n, 1 << 20)
