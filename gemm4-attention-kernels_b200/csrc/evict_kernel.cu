@@ -17,7 +17,7 @@
 //
 // Copy. The kept slots' head rows are laid end to end; a warp takes four of them of one tensor, whose places four of its
 // lanes look up side by side, and has all four in flight, 16 bytes per lane. Nothing is read or written that does not
-// move. It is bound by HBM: 2 * heads_kv KB read and written per slot (8 sequences of up to 16384 slots cut to 4096: 97 us
+// move. It is bound by HBM: 2 * heads_kv KB read and written per slot (8 sequences of up to 16384 slots cut to 4096: 99 us
 // in all, of which the copy's bytes take 82).
 #include <cooperative_groups.h>
 

@@ -10,9 +10,9 @@
 // ridge. So the kernel is built around the stream of cache rows: one CTA per SM, four producer warps that keep two rings
 // of 32-row stages (keys, values) full with one 1 KB bulk copy per row (a page of any size and a row of any page are then
 // the same thing: no tile has to match a page). One producer warp alone can issue such a copy every 74 cycles, 59 % of
-// the bandwidth. Measured: 1 x 131072 keys, 4 KV heads, 8 rows each: 158 us, 6.8 TB/s; 32 sequences of up to 8192: 207 us,
-// 6.7 TB/s (a plain copy moves 6.6). With 32 rows (4 tokens) a tile's instructions cost as much as its bytes: 107 us
-// where the stream alone takes 94 and the bytes 81.
+// the bandwidth. Measured (replays of a graph): 1 x 131072 keys, 4 KV heads, 8 rows each: 158 us, 6.8 TB/s; 32 sequences of
+// up to 8192: 209 us, 6.7 TB/s (a plain copy moves 6.6). With 32 rows (4 tokens) a tile's instructions cost as much as its
+// bytes: 107 us where the stream alone takes 94 and the bytes 81.
 //
 // Split. The (sequence, KV head, row block) units are laid end to end, in tiles of 32 keys, and every CTA takes an
 // equal share of the whole line, whatever the lengths are; the lengths never leave the device. A unit that lies inside
@@ -28,7 +28,7 @@
 //
 // Roundings. The matrix instruction multiplies V, which is exact, by P in V's 16-bit type. P is kept as the sum of TWO such
 // numbers (two products): a single one would put an error of the size of the output's own rounding on top of it. Two
-// leave a weight off by 2^-16 of itself in bf16 and by 2^-22 in fp16, a 128th and a 1024th of the output's rounding; three
+// leave a weight off by 2^-16 of itself in bf16 and by 2^-22 in fp16, a 256th and a 2048th of the output's rounding; three
 // would cost a third product for an error that the scores' own sums in 32 bits have as well. The weights are at most 1, and
 // fp16 ends at 2^-24, so there P is 2^16 times the weight, taken out again where l divides: what a weight loses is then at
 // most 2^-41 of the row's largest one (without the factor, 131071 keys at 2^-26 of one whose value is 0 came out as 0).
@@ -60,7 +60,9 @@ constexpr int kPPitch = 20;                    // 32-bit words per row of P (32 
 constexpr int kMaxRows = 32;                   // rows of a row block
 
 // From 17 rows on some warps need more registers than a block's threads can have each (512: 128, 640: 96), and the others
-// give up some of theirs. The launch checks that the block comes with at least as many as the shares together.
+// give up some of theirs. The launch checks that the block comes with at least as many as the shares together. With 32 rows
+// the compiler still keeps 96 bytes of a thread in local memory (200 bytes loaded): it allots 96 registers to all roles.
+// Splits of 40 / 112 / 104 and 48 / 112 / 104 were no faster.
 template <int kNB>
 constexpr bool kSplitRegs = kNB >= 3;
 template <int kNB>

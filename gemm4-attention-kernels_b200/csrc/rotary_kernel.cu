@@ -12,9 +12,9 @@
 //
 // What bounds it. 2 bytes in and 2 out per element, a handful of operations: HBM. One warp takes a token and a run of
 // its heads; a lane holds the two 16-byte pieces of a head row that belong together, so that both halves of a pair are
-// in its registers, and asks for four head rows before it uses the first. Measured: 2 x 8192 tokens, 36 heads: 193 us a
+// in its registers, and asks for four head rows before it uses the first. Measured: 2 x 8192 tokens, 36 heads: 194 us a
 // direction, 6.2 TB/s, 95 % of a plain copy's rate (212 us where the halves start at no 16-byte boundary and rows go
-// through shared memory); 24576 tokens into a cache, 40 heads: 229 us, 6.3 TB/s.
+// through shared memory); 24576 tokens into a cache, 40 heads: 230 us, 6.3 TB/s.
 #include <cstring>
 
 #include "launch.cuh"
@@ -267,10 +267,11 @@ int launch_rotary_kernel(RotaryParams& p, bool fp16, bool interleaved, cudaStrea
   const int heads = p.heads_q + p.heads_k + p.heads_v;
   // Up to 20 heads per warp, in rounds of four and equal runs where the number of heads allows it: a warp's angles cost as
   // much as five of its heads, and much longer runs leave a tail (37 x 46 tokens, 40 heads: 25 us with two runs, 33 us with
-  // three of 14, 34 us with ten of 4; 2 x 8192 tokens, 36 heads: 193 us with three runs, 201 us with two of 18). Shorter
+  // three of 14, 34 us with ten of 4; 2 x 8192 tokens, 36 heads: 194 us with three runs, 201 us with two of 18). Shorter
   // runs when there would not be half as many warps as the GPU holds (6 x 103 tokens, 36 heads: 11 us with three runs, 13
   // us with two), but four heads, one round of loads, at least. Calls of up to one wave of blocks get the registers of two
-  // blocks per SM (64 tokens: 5.7 us, 6.5 us with three), longer ones three blocks (2 x 8192 tokens: 195 us, 201 us with
+  // blocks per SM (64 tokens: 5.7 us, 6.5 us with three), longer ones three blocks (2 x 8192 tokens: 194 us, 201 us with
+  // two), whose 80 registers a thread leave 32 to 36 bytes of it in local memory (102 to 114 registers, and none there, with
   // two).
   const int64_t half_full = sm_count() * (3 * rot::kWarps) / 2;
   int64_t groups = (heads + 19) / 20;

@@ -4,9 +4,10 @@ fills it and the eviction that shortens it (no counterpart in the reference, whi
 A cache is two tensors ``k_pages`` and ``v_pages`` of shape (num_pages, page_size, heads_kv, 512), bf16 or fp16, any page
 size. ``page_table`` (B, max_pages) int32 names the pages of each sequence, ``seqlens_k`` (B,) int32 the slots in use;
 slot j of sequence b is row ``j % page_size`` of page ``page_table[b, j // page_size]``. Both stay on the device: no call
-here waits for the GPU, and all of them can be captured in a CUDA graph. The kernels check every page id and length
-before they use it; ``kernel_status()`` is 107 or 108 after a call that named a page the cache does not have or a
-sequence longer than its row of the table.
+here waits for the GPU, and all of them can be captured in a CUDA graph, with one exception: an append of packed tokens
+reads ``cu_seqlens_q`` back to check it, unless ``cu_seqlens_validation(False)`` is in force. The kernels check every page
+id and length before they use it; ``kernel_status()`` is 107 or 108 after a call that named a page the cache does not have
+or a sequence longer than its row of the table (or than its weights).
 
 One step of a decoder's layer::
 
@@ -263,10 +264,11 @@ def split_flash_attn_paged_func(
     are not read, and one that only some rows may see leaves the others alone, whatever it holds.
 
     ``key_weights`` (B, slots) float32, optional: every slot's softmax weight, summed over all query heads and tokens,
-    is added to it in place, in a fixed order (what ``split_paged_evict_func`` ranks by). Costs a workspace of
-    Hq * Sq * 4 bytes per slot of it.
+    is added to it in place, in a fixed order (what ``split_paged_evict_func`` ranks by). Slots behind its end are not
+    counted (status 108). Costs a workspace of Hq * Sq * 4 bytes per slot of it.
 
-    The cache is read once for up to 32 rows (Sq * Hq / heads_kv); more rows take as many passes.
+    The cache is read once for up to 32 rows (Sq * Hq / heads_kv); more rows take as many passes. In fp16 a weight loses up
+    to 2^-41 of its row's largest one in the output.
     """
     if not isinstance(window_size, tuple) or len(window_size) != 2:
         raise TypeError("window_size must be a tuple of (left, right)")
@@ -446,9 +448,10 @@ def split_paged_append_func(
 
     Batched: q (B, S, Hq, 512), k and v (B, S, heads_kv, 512), S new tokens per sequence. Packed: (T, heads, 512) and
     ``cu_seqlens_q`` int32 of B + 1 entries, any number of tokens per sequence (its values are checked as in
-    ``split_flash_attn_varlen_func``; ``cu_seqlens_validation(False)`` leaves that out). ``seqlens_k[b]`` is the length
-    of sequence b WITH its new tokens, which fill its last slots. Tokens whose slot would be negative are not stored
-    (length 0: a row that only pads the batch); two tokens must not share a slot.
+    ``split_flash_attn_varlen_func``, which waits for the GPU and cannot be captured; ``cu_seqlens_validation(False)``
+    leaves that out). ``seqlens_k[b]`` is the length of sequence b WITH its new tokens, which fill its last slots. Tokens
+    whose slot would be negative are not stored (length 0: a row that only pads the batch); two tokens must not share a
+    slot, nor ``k_pages`` and ``v_pages`` memory.
 
     ``inv_freq``, ``interleaved``, ``factor``: as in ``split_rotary_func``; without ``inv_freq`` nothing is rotated.
     Positions are the slots, unless ``positions`` (one per token, int32 or int64) says otherwise, as it has to after an
